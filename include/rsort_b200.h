@@ -506,6 +506,134 @@ rsort_status rsort_gather_segments(unsigned nseg, const void *const *d_src, cons
 rsort_status rsort_keys_static(rsort_key_t key, int descending, void *d_keys, size_t n,
                                rsort_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Expert routing (no reference counterpart): token slots sorted by expert,
+ * rows gathered into expert order, expert outputs combined back with their
+ * weights, and the gradients of both.
+ *
+ * Slot s = token * top_k + k holds the expert id of the token's k-th choice.
+ * Ids outside 0..experts-1 are dropped slots (padding tokens, experts of
+ * another rank).  rsort_expert_sort places the slots stably by expert:
+ *   counts[e]       slots of expert e
+ *   offsets[e]      first row of expert e; every expert's segment is padded to
+ *                   a multiple of `align` rows, offsets[experts] ends the last
+ *   row_of_slot[s]  the slot's row, -1 when it was dropped
+ *   slot_of_row[r]  the row's slot, -1 in padding and behind the last segment
+ * The plan stays on the device: nothing synchronizes, so it can be captured.
+ * rsort_expert_rows(nslots, experts, align) rows hold any outcome (0: the
+ * sizes are not supported; at most RSORT_MAX_EXPERTS experts, an align of at
+ * most RSORT_MAX_EXPERT_ALIGN and 2^31 - 1 rows).  d_scratch holds
+ * rsort_expert_sort_scratch_bytes(nslots, experts) bytes, 4-byte aligned, and
+ * serves one call at a time.
+ *
+ *   rsort_expert_gather   rows[row_of_slot[t, k]] = x[t] for every kept slot
+ *                         (rows of row_bytes, strides in bytes); with
+ *                         zero_padding the padding rows of the segments become
+ *                         zeros.  Rows behind the last segment are left as
+ *                         they are.
+ *   rsort_expert_combine  out[t] = sum over k of weights[t, k] *
+ *                         rows[row_of_slot[t, k]], in fp32 in the order of k,
+ *                         rounded once; 0 for a token without kept slots.
+ *                         Null weights count as 1: that is the gradient of
+ *                         rsort_expert_gather.
+ *   rsort_expert_combine_backward
+ *                         grad_rows[row_of_slot[t, k]] = weights[t, k] *
+ *                         grad_out[t] (padding rows as in the gather) and
+ *                         grad_weights[t, k] = <grad_out[t],
+ *                         rows[row_of_slot[t, k]]> in fp32, 0 for dropped
+ *                         slots.  Either output may be null.
+ * Row types are f32, f16 or bf16, weights any of them (tokens x top_k,
+ * contiguous); strides of typed rows are in elements.  Input rows may have any
+ * stride (0: one row for all); output rows must not overlap one another or an
+ * input.  `rows` and `grad_rows` hold nrows rows.
+ * ------------------------------------------------------------------------- */
+#define RSORT_MAX_EXPERTS 1024
+#define RSORT_MAX_EXPERT_ALIGN 65536
+
+typedef struct {
+    const int32_t *row_of_slot; /* tokens * top_k */
+    const int32_t *offsets;     /* experts + 1 */
+    const int32_t *counts;      /* experts */
+    size_t tokens, top_k, experts, nrows;
+} rsort_expert_plan;
+
+size_t rsort_expert_rows(size_t nslots, size_t experts, size_t align);
+size_t rsort_expert_sort_scratch_bytes(size_t nslots, size_t experts);
+rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t nslots,
+                               size_t experts, size_t align, int32_t *d_row_of_slot,
+                               int32_t *d_slot_of_row, size_t nrows, int32_t *d_offsets,
+                               int32_t *d_counts, void *d_scratch, size_t scratch_bytes,
+                               rsort_stream_t stream);
+rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x, size_t x_stride,
+                                 void *d_rows, size_t rows_stride, size_t row_bytes,
+                                 int zero_padding, rsort_stream_t stream);
+rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t type,
+                                  const void *d_rows, size_t rows_stride, const void *d_weights,
+                                  rsort_key_t weight_type, void *d_out, size_t out_stride,
+                                  size_t width, rsort_stream_t stream);
+rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_key_t type,
+                                           const void *d_grad_out, size_t grad_out_stride,
+                                           const void *d_rows, size_t rows_stride,
+                                           const void *d_weights, rsort_key_t weight_type,
+                                           void *d_grad_rows, size_t grad_rows_stride,
+                                           void *d_grad_weights, size_t width, int zero_padding,
+                                           rsort_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Cache eviction by accumulated attention weight (no reference counterpart).
+ *
+ * A cache holds `capacity` positions for each of batch x heads; the first
+ * lengths[b] (clamped to 0..capacity) are in use.  batch * heads <= 65535.
+ *
+ *   rsort_attention_weight_add
+ *       scores[b, h, s] = decay * scores[b, h, s] + the sum of
+ *       weights[b, h * group + g, q, s] over g < group and q < queries, in
+ *       fp32, for s < lengths[b]; other totals are left as they are.  With
+ *       causal the queries are the last ones of the sequence: query q sees
+ *       s <= lengths[b] - queries + q, and what it does not see is not read.
+ *       Weights are f32, f16 or bf16; strides in elements, positions next to
+ *       one another.  Null lengths: every position is in use.
+ *   rsort_cache_select
+ *       kept[b, h, 0..budget-1]: the positions that stay, ascending, then -1;
+ *       kept_lengths[b] = min(lengths[b], budget).  A sequence of at most
+ *       `budget` positions keeps them all.  Otherwise the first `sinks`, the
+ *       last `recent` and the heaviest of those between stay; equal totals
+ *       keep the lower position, NaN counts as -inf, -0 as +0.
+ *   rsort_cache_compact
+ *       dst[b, h, j] = src[b, h, kept[b, h, j]] for j < kept_lengths[b], for
+ *       up to RSORT_MAX_CACHES arrays of rows in one launch (keys, values,
+ *       totals, scales).  Later rows are left as they are.  src == dst (with
+ *       equal strides, for all arrays) compacts in place and takes ascending
+ *       kept positions, as rsort_cache_select writes them; otherwise no dst
+ *       may overlap a src.  Positions outside 0..capacity-1 are skipped.
+ *       Strides are in bytes, a row's bytes are next to one another.
+ * ------------------------------------------------------------------------- */
+#define RSORT_MAX_CACHES 8
+
+typedef struct {
+    const void *src;
+    void *dst;
+    size_t row_bytes;
+    size_t src_stride_b, src_stride_h, src_stride_s;
+    size_t dst_stride_b, dst_stride_h, dst_stride_s;
+} rsort_cache_rows;
+
+rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights, size_t stride_b,
+                                        size_t stride_h, size_t stride_q, size_t batch,
+                                        size_t heads, size_t group, size_t queries,
+                                        size_t capacity, const int32_t *d_lengths, float decay,
+                                        int causal, float *d_scores, size_t score_stride_b,
+                                        size_t score_stride_h, rsort_stream_t stream);
+rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
+                                size_t score_stride_h, const int32_t *d_lengths, size_t batch,
+                                size_t heads, size_t capacity, size_t budget, size_t sinks,
+                                size_t recent, int32_t *d_kept, int32_t *d_kept_lengths,
+                                rsort_stream_t stream);
+rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
+                                 const int32_t *d_kept, const int32_t *d_kept_lengths,
+                                 size_t batch, size_t heads, size_t budget, size_t capacity,
+                                 rsort_stream_t stream);
+
 const char *rsort_status_string(rsort_status status);
 void rsort_last_error(rsort_error_info *out);
 
@@ -521,7 +649,9 @@ enum { RSORT_KERNEL_INIT = 0, RSORT_KERNEL_HISTOGRAM = 1, RSORT_KERNEL_ONESWEEP 
        /* the uniform-step form of a pass after the first (4- and 8-byte keys):
         * it sorts passes where runs of equal keys are expected and exits at
         * once elsewhere, so a pass costs this launch plus the onesweep launch */
-       RSORT_KERNEL_ONESWEEP_RUNS = 8 };
+       RSORT_KERNEL_ONESWEEP_RUNS = 8,
+       /* expert sort; expert gather, combine and gradients; cache eviction */
+       RSORT_KERNEL_EXPERT_SORT = 9, RSORT_KERNEL_EXPERT_ROWS = 10, RSORT_KERNEL_CACHE = 11 };
 
 /* Benchmark instrumentation (no reference counterpart): while enabled, every
  * kernel launch of the calling host thread is bracketed by CUDA events on its

@@ -6,6 +6,8 @@ Modules:
   cub     -- rccl-cub DeviceRadixSort functions, workspaces and DoubleBuffer
   thrust  -- rccl-thrust sort()/sort_unstable()/with_values() radix lowering
   dist    -- multi-GPU sample sort (torch.distributed over NCCL)
+  experts -- token slots sorted by expert, rows moved there and back, gradients
+  eviction -- cache positions scored, selected and compacted
   errors  -- DeviceAlgorithmError mirror
 """
 from . import errors

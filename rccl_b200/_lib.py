@@ -30,7 +30,8 @@ RSORT_BAD_ARGUMENT = 8
 
 # kernel ids of rsort_profile_read
 KERNEL_NAMES = {0: "init", 1: "histogram", 2: "onesweep", 3: "single_tile", 4: "dist",
-                5: "merge", 6: "gather", 7: "records", 8: "onesweep_runs"}
+                5: "merge", 6: "gather", 7: "records", 8: "onesweep_runs",
+                9: "expert_sort", 10: "expert_rows", 11: "cache"}
 IPC_HANDLE_BYTES = 64
 GATHER_MAX_SEGMENTS = 64
 MAX_ITEMS = 1 << 40  # RSORT_MAX_ITEMS
@@ -77,6 +78,15 @@ EXPORTED_SYMBOLS = (
     "rsort_merge_multiway",
     "rsort_sort_by_scratch_bytes",
     "rsort_sort_by",
+    "rsort_expert_rows",
+    "rsort_expert_sort_scratch_bytes",
+    "rsort_expert_sort",
+    "rsort_expert_gather",
+    "rsort_expert_combine",
+    "rsort_expert_combine_backward",
+    "rsort_attention_weight_add",
+    "rsort_cache_select",
+    "rsort_cache_compact",
 )
 
 # rsort_exchange_t
@@ -94,6 +104,29 @@ class CompareTerm(ctypes.Structure):
     _fields_ = [("offset", ctypes.c_uint32), ("type", ctypes.c_int32),
                 ("projection", ctypes.c_int32), ("order", ctypes.c_int32),
                 ("operand", ctypes.c_int64)]
+
+
+# limits of the expert routing and the cache eviction
+MAX_EXPERTS = 1024
+MAX_EXPERT_ALIGN = 65536
+MAX_CACHES = 8
+
+
+class ExpertPlanArgs(ctypes.Structure):
+    """rsort_expert_plan"""
+    _fields_ = [("row_of_slot", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("counts", ctypes.c_void_p), ("tokens", ctypes.c_size_t),
+                ("top_k", ctypes.c_size_t), ("experts", ctypes.c_size_t),
+                ("nrows", ctypes.c_size_t)]
+
+
+class CacheRows(ctypes.Structure):
+    """rsort_cache_rows"""
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p),
+                ("row_bytes", ctypes.c_size_t), ("src_stride_b", ctypes.c_size_t),
+                ("src_stride_h", ctypes.c_size_t), ("src_stride_s", ctypes.c_size_t),
+                ("dst_stride_b", ctypes.c_size_t), ("dst_stride_h", ctypes.c_size_t),
+                ("dst_stride_s", ctypes.c_size_t)]
 
 
 class Controls(ctypes.Structure):
@@ -208,6 +241,27 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.rsort_multiway_scratch_bytes.restype = sz
     lib.rsort_merge_multiway.argtypes = [i, i, u, pvp, pvp, psz, sz, vp, vp, vp, sz, vp]
     lib.rsort_merge_multiway.restype = i
+    plan = ctypes.POINTER(ExpertPlanArgs)
+    lib.rsort_expert_rows.argtypes = [sz, sz, sz]
+    lib.rsort_expert_rows.restype = sz
+    lib.rsort_expert_sort_scratch_bytes.argtypes = [sz, sz]
+    lib.rsort_expert_sort_scratch_bytes.restype = sz
+    lib.rsort_expert_sort.argtypes = [i, vp, sz, sz, sz, vp, vp, sz, vp, vp, vp, sz, vp]
+    lib.rsort_expert_sort.restype = i
+    lib.rsort_expert_gather.argtypes = [plan, vp, sz, vp, sz, sz, i, vp]
+    lib.rsort_expert_gather.restype = i
+    lib.rsort_expert_combine.argtypes = [plan, i, vp, sz, vp, i, vp, sz, sz, vp]
+    lib.rsort_expert_combine.restype = i
+    lib.rsort_expert_combine_backward.argtypes = [plan, i, vp, sz, vp, sz, vp, i, vp, sz, vp, sz,
+                                                  i, vp]
+    lib.rsort_expert_combine_backward.restype = i
+    lib.rsort_attention_weight_add.argtypes = [i, vp, sz, sz, sz, sz, sz, sz, sz, sz, vp,
+                                               ctypes.c_float, i, vp, sz, sz, vp]
+    lib.rsort_attention_weight_add.restype = i
+    lib.rsort_cache_select.argtypes = [vp, sz, sz, vp, sz, sz, sz, sz, sz, sz, vp, vp, vp]
+    lib.rsort_cache_select.restype = i
+    lib.rsort_cache_compact.argtypes = [ctypes.POINTER(CacheRows), sz, vp, vp, sz, sz, sz, sz, vp]
+    lib.rsort_cache_compact.restype = i
 
 
 def lib() -> ctypes.CDLL:

@@ -1,0 +1,564 @@
+// Cache eviction by accumulated attention weight: totals of the attention
+// weights per cached position, the heaviest positions of every head, and the
+// cache's rows moved together.
+//
+// A cache holds `capacity` positions for each of batch x heads rows; the first
+// lengths[b] of them are in use.
+#include <climits>
+
+#include "../../include/rsort_b200.h"
+#include "rsort_device.cuh"
+#include "rsort_internal.cuh"
+#include "rsort_rows.cuh"
+
+using namespace rsort;
+
+namespace {
+
+__device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t b,
+                                              uint32_t capacity) {
+    if (!lengths) return capacity;
+    const int32_t n = lengths[b];
+    return n < 0 ? 0u : min(uint32_t(n), capacity);
+}
+
+// ---------------------------------------------------------------------------
+// Totals of attention weights
+// ---------------------------------------------------------------------------
+constexpr int ADD_BLOCK = 256;
+
+struct AddArgs {
+    const void *weights;
+    size_t stride_b, stride_h, stride_q;  // elements
+    float *scores;
+    size_t score_b, score_h;
+    const int32_t *lengths;
+    uint32_t heads, group, queries, capacity;
+    float decay;
+    int causal;
+};
+
+// One thread sums V neighbouring positions over the group's heads and the
+// queries, in fp32.
+template <typename T, int V>
+__global__ void __launch_bounds__(ADD_BLOCK) weight_add_kernel(const AddArgs a) {
+    const uint32_t b = blockIdx.y / a.heads, h = blockIdx.y % a.heads;
+    const uint32_t n = length_of(a.lengths, b, a.capacity);
+    const uint32_t s0 = (blockIdx.x * ADD_BLOCK + threadIdx.x) * V;
+    if (s0 >= n) return;
+    float acc[V] = {};
+    // Query q sees the positions below n - queries + q + 1.
+    const int64_t hidden = a.causal ? int64_t(s0) - (int64_t(n) - a.queries) : 0;
+    const uint32_t q0 = hidden <= 0 ? 0 : uint32_t(hidden);
+    for (uint32_t g = 0; g < a.group; ++g) {
+        const T *w = static_cast<const T *>(a.weights) + b * a.stride_b +
+                     (size_t(h) * a.group + g) * a.stride_h + s0;
+        for (uint32_t q = q0; q < a.queries; ++q) {
+            const uint32_t end = a.causal ? n - a.queries + q + 1 : n;
+            const T *p = w + q * a.stride_q;
+            if (s0 + V <= end) {
+                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(p);
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += to_float(v.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (s0 + i < end) acc[i] += to_float(p[i]);
+            }
+        }
+    }
+    float *out = a.scores + b * a.score_b + h * a.score_h + s0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (s0 + i < n) out[i] = fmaf(a.decay, out[i], acc[i]);
+}
+
+// ---------------------------------------------------------------------------
+// Selection
+// ---------------------------------------------------------------------------
+constexpr int SELECT_BLOCK = 512;
+constexpr int SELECT_WARPS = SELECT_BLOCK / 32;
+
+struct SelectArgs {
+    const float *scores;
+    size_t score_b, score_h;
+    const int32_t *lengths;
+    uint32_t heads, capacity, budget, sinks, recent;
+    int32_t *kept, *kept_lengths;
+};
+
+// Order image of a total: ascending as unsigned, -0 as +0, NaN as -inf.
+__device__ __forceinline__ uint32_t score_image(float x) {
+    x = x != x ? -INFINITY : x + 0.0f;
+    const uint32_t u = __float_as_uint(x);
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+
+// Exclusive sum over the block of one value a thread; *total gets the sum.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= uint32_t(off)) inc += y;
+    }
+    __syncthreads();  // warp_sums of an earlier scan have been read
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < SELECT_WARPS; ++w) {
+        const uint32_t s = warp_sums[w];
+        if (uint32_t(w) < warp) before += s;
+        all += s;
+    }
+    *total = all;
+    return before + inc - v;
+}
+
+// One CTA a head: radix selection of the smallest kept image, eight bits a
+// pass, then one ordered pass that writes the kept positions.
+__global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const SelectArgs a) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t warp_sums[SELECT_WARPS];
+    __shared__ uint32_t chosen, left;
+    const uint32_t b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, tid = threadIdx.x;
+    const uint32_t n = length_of(a.lengths, b, a.capacity);
+    int32_t *kept = a.kept + size_t(blockIdx.x) * a.budget;
+    if (h == 0 && tid == 0) a.kept_lengths[b] = int32_t(min(n, a.budget));
+    if (n <= a.budget) {
+        for (uint32_t j = tid; j < a.budget; j += SELECT_BLOCK) kept[j] = j < n ? int32_t(j) : -1;
+        return;
+    }
+    for (uint32_t j = tid; j < a.sinks; j += SELECT_BLOCK) kept[j] = int32_t(j);
+    for (uint32_t j = tid; j < a.recent; j += SELECT_BLOCK)
+        kept[a.budget - a.recent + j] = int32_t(n - a.recent + j);
+    const uint32_t need = a.budget - a.sinks - a.recent;
+    if (need == 0) return;
+    const float *scores = a.scores + b * a.score_b + h * a.score_h + a.sinks;
+    const uint32_t m = n - a.sinks - a.recent;  // more than need
+    uint32_t prefix = 0, want = need;  // of the images that start with prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (uint32_t i = tid; i < 256; i += SELECT_BLOCK) hist[i] = 0;
+        __syncthreads();
+        const uint32_t above = shift == 24 ? 0 : 0xffffffffu << (shift + 8);
+        for (uint32_t i = tid; i < m; i += SELECT_BLOCK) {
+            const uint32_t v = score_image(scores[i]);
+            if ((v & above) == prefix) atomicAdd(&hist[(v >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        // From the highest digit down: the digit in which the count of kept
+        // images is reached.
+        const uint32_t d = 255 - tid;
+        const uint32_t v = tid < 256 ? hist[d] : 0;
+        uint32_t total;
+        const uint32_t higher = block_scan(v, warp_sums, &total);
+        if (tid < 256 && higher < want && want <= higher + v) {
+            chosen = d;
+            left = want - higher;
+        }
+        __syncthreads();
+        prefix |= chosen << shift;
+        want = left;
+    }
+    // prefix is the smallest kept image; `want` of its equals stay, the lowest
+    // positions first.
+    int32_t *out = kept + a.sinks;
+    uint32_t done = 0, equals = 0;
+    for (uint32_t i0 = 0; i0 < m; i0 += SELECT_BLOCK) {
+        const uint32_t i = i0 + tid;
+        const uint32_t v = i < m ? score_image(scores[i]) : 0;
+        const bool eq = i < m && v == prefix;
+        uint32_t total;
+        const uint32_t rank = equals + block_scan(eq ? 1 : 0, warp_sums, &total);
+        equals += total;
+        const bool keep = i < m && (v > prefix || (eq && rank < want));
+        const uint32_t at = done + block_scan(keep ? 1 : 0, warp_sums, &total);
+        done += total;
+        if (keep && at < need) out[at] = int32_t(a.sinks + i);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Moving the cache's rows
+// ---------------------------------------------------------------------------
+constexpr int MOVE_BLOCK = 256;
+
+struct Rows {
+    const char *src;
+    char *dst;
+    size_t src_b, src_h, src_s, dst_b, dst_h, dst_s;  // bytes
+    uint32_t units, access;  // accesses of `access` bytes in a row
+    uint32_t slices;         // in place: CTAs that share a row's accesses
+    uint32_t first_block;
+};
+
+struct MoveArgs {
+    Rows rows[RSORT_MAX_CACHES];
+    uint32_t count, batch, heads, budget, capacity;
+    const int32_t *kept, *kept_lengths;
+};
+
+// A kept position; -1 unless it can be read.
+__device__ __forceinline__ int32_t kept_at(const int32_t *kept, uint32_t j, uint32_t capacity) {
+    const int32_t p = kept[j];
+    return uint32_t(p) < capacity ? p : -1;
+}
+
+// Out of place: the accesses of MOVE_BLOCK * MOVE_STEPS row units a CTA.
+constexpr int MOVE_STEPS = 4;
+
+template <typename U>
+__device__ __forceinline__ void move_out(const Rows &r, const int32_t *kept, const char *src,
+                                         char *dst, uint32_t n, uint32_t capacity, uint64_t first) {
+    const uint64_t total = uint64_t(n) * r.units;
+#pragma unroll
+    for (int k = 0; k < MOVE_STEPS; ++k) {
+        const uint64_t i = first + uint64_t(k) * MOVE_BLOCK + threadIdx.x;
+        if (i >= total) return;
+        const uint32_t j = uint32_t(i / r.units), u = uint32_t(i - uint64_t(j) * r.units);
+        const int32_t p = kept_at(kept, j, capacity);
+        if (p < 0) continue;
+        reinterpret_cast<U *>(dst + size_t(j) * r.dst_s)[u] =
+            reinterpret_cast<const U *>(src + size_t(p) * r.src_s)[u];
+    }
+}
+
+__device__ __forceinline__ const Rows &rows_of_block(const MoveArgs &a, uint32_t *block) {
+    uint32_t t = 0;
+    while (t + 1 < a.count && blockIdx.x >= a.rows[t + 1].first_block) ++t;
+    *block = blockIdx.x - a.rows[t].first_block;
+    return a.rows[t];
+}
+
+__global__ void __launch_bounds__(MOVE_BLOCK)
+    cache_move_kernel(const __grid_constant__ MoveArgs a) {
+    uint32_t block;
+    const Rows &r = rows_of_block(a, &block);
+    const uint32_t bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
+    const uint32_t n = min(length_of(a.kept_lengths, b, a.budget), a.capacity);
+    const int32_t *kept = a.kept + size_t(bh) * a.budget;
+    const char *src = r.src + b * r.src_b + h * r.src_h;
+    char *dst = r.dst + b * r.dst_b + h * r.dst_h;
+    const uint64_t first = uint64_t(block) * (MOVE_BLOCK * MOVE_STEPS);
+    switch (r.access) {
+        case 16: move_out<uint4>(r, kept, src, dst, n, a.capacity, first); break;
+        case 8: move_out<uint2>(r, kept, src, dst, n, a.capacity, first); break;
+        case 4: move_out<uint32_t>(r, kept, src, dst, n, a.capacity, first); break;
+        case 2: move_out<uint16_t>(r, kept, src, dst, n, a.capacity, first); break;
+        default: move_out<uint8_t>(r, kept, src, dst, n, a.capacity, first); break;
+    }
+}
+
+// In place: one CTA walks all rows of a slice of the row's accesses in order.
+// kept[j] >= j, so what a step reads was not written by the steps before it;
+// a barrier lets every read of a step come before its writes.
+template <typename U>
+__device__ __forceinline__ void move_in_place(const Rows &r, const int32_t *kept, char *rows,
+                                              uint32_t n, uint32_t capacity, uint32_t slice) {
+    const uint32_t per = (r.units + r.slices - 1) / r.slices;
+    const uint32_t u0 = slice * per, u1 = min(u0 + per, r.units);
+    if (u0 >= u1) return;
+    const uint64_t total = uint64_t(n) * (u1 - u0);
+    for (uint64_t i0 = 0; i0 < total; i0 += MOVE_BLOCK * MOVE_STEPS) {
+        U v[MOVE_STEPS];
+        U *to[MOVE_STEPS];
+#pragma unroll
+        for (int k = 0; k < MOVE_STEPS; ++k) {
+            const uint64_t i = i0 + uint64_t(k) * MOVE_BLOCK + threadIdx.x;
+            to[k] = nullptr;
+            if (i < total) {
+                const uint32_t j = uint32_t(i / (u1 - u0));
+                const uint32_t u = u0 + uint32_t(i - uint64_t(j) * (u1 - u0));
+                const int32_t p = kept_at(kept, j, capacity);
+                if (p > int32_t(j)) {
+                    v[k] = reinterpret_cast<const U *>(rows + size_t(p) * r.src_s)[u];
+                    to[k] = reinterpret_cast<U *>(rows + size_t(j) * r.src_s) + u;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < MOVE_STEPS; ++k)
+            if (to[k]) *to[k] = v[k];
+    }
+}
+
+__global__ void __launch_bounds__(MOVE_BLOCK)
+    cache_move_in_place_kernel(const __grid_constant__ MoveArgs a) {
+    uint32_t slice;
+    const Rows &r = rows_of_block(a, &slice);
+    const uint32_t bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
+    const uint32_t n = min(length_of(a.kept_lengths, b, a.budget), a.capacity);
+    const int32_t *kept = a.kept + size_t(bh) * a.budget;
+    char *rows = r.dst + b * r.dst_b + h * r.dst_h;
+    switch (r.access) {
+        case 16: move_in_place<uint4>(r, kept, rows, n, a.capacity, slice); break;
+        case 8: move_in_place<uint2>(r, kept, rows, n, a.capacity, slice); break;
+        case 4: move_in_place<uint32_t>(r, kept, rows, n, a.capacity, slice); break;
+        case 2: move_in_place<uint16_t>(r, kept, rows, n, a.capacity, slice); break;
+        default: move_in_place<uint8_t>(r, kept, rows, n, a.capacity, slice); break;
+    }
+}
+
+// batch x heads is a grid dimension of at most 65535.
+rsort_status check_grid(size_t batch, size_t heads, size_t capacity) {
+    if (batch > 65535 || heads > 65535 || batch * heads > 65535)
+        return fail(RSORT_SIZE_OVERFLOW, "cache batch times heads", 65535, batch * heads);
+    if (capacity > size_t(INT_MAX) - 1)
+        return fail(RSORT_SIZE_OVERFLOW, "cache capacity (32-bit positions)");
+    return RSORT_OK;
+}
+
+// A strided [batch, heads, positions] array of `bytes`-wide items; strides in
+// bytes, dimensions of one entry dropped, smallest stride first.
+struct Strided {
+    uintptr_t base;
+    size_t bytes;
+    size_t stride[3], count[3];
+    int dims;
+    ByteRange range;
+};
+
+// False when an offset could wrap.
+bool strided(const void *p, size_t batch, size_t heads, size_t n, size_t sb, size_t sh, size_t ss,
+             size_t bytes, Strided *out) {
+    if (!rows_fit(batch, sb, bytes) || !rows_fit(heads, sh, bytes) || !rows_fit(n, ss, bytes))
+        return false;
+    const size_t stride[3] = {ss, sh, sb}, count[3] = {n, heads, batch};
+    Strided r{addr(p), bytes, {}, {}, 0, {}};
+    size_t extent = bytes;
+    for (int i = 0; i < 3; ++i) {
+        if (count[i] <= 1) continue;
+        int at = r.dims++;
+        for (; at > 0 && r.stride[at - 1] > stride[i]; --at) {
+            r.stride[at] = r.stride[at - 1];
+            r.count[at] = r.count[at - 1];
+        }
+        r.stride[at] = stride[i];
+        r.count[at] = count[i];
+        extent += (count[i] - 1) * stride[i];
+    }
+    r.range = {r.base, r.base + extent};
+    *out = r;
+    return true;
+}
+
+// No two items share a byte (sufficient: every stride spans what lies inside).
+bool items_apart(const Strided &a) {
+    size_t inner = a.bytes;
+    for (int i = 0; i < a.dims; ++i) {
+        if (a.stride[i] < inner) return false;
+        inner += (a.count[i] - 1) * a.stride[i];
+    }
+    return true;
+}
+
+// No item of one shares a byte with an item of the other (sufficient: their
+// ranges are apart, or both have the same strides and interleave, as the keys
+// and values of one packed allocation do).
+bool arrays_apart(const Strided &a, const Strided &b) {
+    if (!overlap(a.range, b.range)) return true;
+    if (a.dims != b.dims || a.bytes != b.bytes) return false;
+    for (int i = 0; i < a.dims; ++i)
+        if (a.stride[i] != b.stride[i]) return false;
+    const size_t d = a.base < b.base ? b.base - a.base : a.base - b.base;
+    size_t inner = a.bytes;
+    for (int i = 0; i < a.dims; ++i) {
+        // Everything below dimension i lies within `inner` bytes of a multiple
+        // of its stride when the larger strides are multiples of it too.
+        bool multiples = a.stride[i] > 0;
+        for (int j = i + 1; j < a.dims && multiples; ++j) multiples = a.stride[j] % a.stride[i] == 0;
+        if (multiples) {
+            const size_t r = d % a.stride[i];
+            if (r >= inner && r + inner <= a.stride[i]) return true;
+        }
+        inner += ((a.count[i] > b.count[i] ? a.count[i] : b.count[i]) - 1) * a.stride[i];
+    }
+    return false;
+}
+
+}  // namespace
+
+extern "C" {
+
+rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights, size_t stride_b,
+                                        size_t stride_h, size_t stride_q, size_t batch,
+                                        size_t heads, size_t group, size_t queries,
+                                        size_t capacity, const int32_t *d_lengths, float decay,
+                                        int causal, float *d_scores, size_t score_stride_b,
+                                        size_t score_stride_h, rsort_stream_t stream) {
+    const size_t eb = real_bytes(type);
+    if (!eb) return fail(RSORT_BAD_ARGUMENT, "attention weight type (f32, f16 or bf16)");
+    rsort_status st = check_grid(batch, heads, capacity);
+    if (st != RSORT_OK) return st;
+    if (group < 1 || group > size_t(INT_MAX) || queries > size_t(INT_MAX))
+        return fail(RSORT_BAD_ARGUMENT, "attention weight heads per cache head or queries");
+    if (batch == 0 || heads == 0 || capacity == 0) return RSORT_OK;
+    if ((queries && !d_weights) || !d_scores) return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    constexpr size_t most = size_t(1) << 50;
+    if (stride_b > most || stride_h > most || stride_q > most || score_stride_b > most ||
+        score_stride_h > most || !rows_fit(batch, stride_b * eb, 0) ||
+        !rows_fit(heads * group, stride_h * eb, 0) || !rows_fit(queries, stride_q * eb, 0))
+        return fail(RSORT_SIZE_OVERFLOW, "attention weight strides");
+    Strided scores{};
+    if (!strided(d_scores, batch, heads, capacity, score_stride_b * 4, score_stride_h * 4, 4, 4,
+                 &scores))
+        return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
+    if (!items_apart(scores)) return fail(RSORT_BAD_ARGUMENT, "cache score strides overlap");
+    st = check_alignment(addr(d_weights), eb, "attention weights alignment");
+    if (st == RSORT_OK) st = check_alignment(addr(d_scores), 4, "cache scores alignment");
+    if (st == RSORT_OK) st = check_alignment(addr(d_lengths), 4, "cache lengths alignment");
+    if (st != RSORT_OK) return st;
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    AddArgs a{d_weights,         stride_b,       stride_h,        stride_q,
+              d_scores,          score_stride_b, score_stride_h,  d_lengths,
+              uint32_t(heads),   uint32_t(group), uint32_t(queries), uint32_t(capacity),
+              decay,             causal != 0};
+    const size_t access =
+        access_bytes(addr(d_weights) | stride_b * eb | stride_h * eb | stride_q * eb, 16);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    auto go = [&](auto t, auto v) {
+        using T = decltype(t);
+        constexpr int V = decltype(v)::value;
+        const size_t per = size_t(ADD_BLOCK) * V;
+        const dim3 grid(unsigned((capacity + per - 1) / per), unsigned(batch * heads));
+        weight_add_kernel<T, V><<<grid, ADD_BLOCK, 0, s>>>(a);
+        return cudaGetLastError();
+    };
+    LaunchScope scope(RSORT_KERNEL_CACHE, s);
+    return launched(with_type(type, access, go), "attention weight add launch");
+}
+
+rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
+                                size_t score_stride_h, const int32_t *d_lengths, size_t batch,
+                                size_t heads, size_t capacity, size_t budget, size_t sinks,
+                                size_t recent, int32_t *d_kept, int32_t *d_kept_lengths,
+                                rsort_stream_t stream) {
+    rsort_status st = check_grid(batch, heads, capacity);
+    if (st != RSORT_OK) return st;
+    if (budget < 1 || budget > size_t(INT_MAX))
+        return fail(RSORT_BAD_ARGUMENT, "cache budget", 1, budget);
+    if (sinks > budget || recent > budget - sinks)
+        return fail(RSORT_BAD_ARGUMENT, "cache sinks and recent positions exceed the budget",
+                    budget, sinks + recent);
+    if (batch == 0 || heads == 0) return RSORT_OK;
+    if ((capacity && !d_scores) || !d_kept || !d_kept_lengths)
+        return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    constexpr size_t most = size_t(1) << 50;
+    if (score_stride_b > most || score_stride_h > most)
+        return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
+    st = check_alignment(addr(d_scores) | addr(d_lengths) | addr(d_kept) | addr(d_kept_lengths), 4,
+                         "cache selection alignment");
+    if (st != RSORT_OK) return st;
+    if (overlap(rows_range(d_kept_lengths, batch, 4, 4), rows_range(d_lengths, batch, 4, 4)))
+        return fail(RSORT_BAD_ARGUMENT, "kept lengths overlap the lengths");
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    SelectArgs a{d_scores,           score_stride_b,  score_stride_h,  d_lengths,
+                 uint32_t(heads),    uint32_t(capacity), uint32_t(budget), uint32_t(sinks),
+                 uint32_t(recent),   d_kept,          d_kept_lengths};
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    LaunchScope scope(RSORT_KERNEL_CACHE, s);
+    cache_select_kernel<<<unsigned(batch * heads), SELECT_BLOCK, 0, s>>>(a);
+    return launched(cudaGetLastError(), "cache selection launch");
+}
+
+rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
+                                 const int32_t *d_kept, const int32_t *d_kept_lengths,
+                                 size_t batch, size_t heads, size_t budget, size_t capacity,
+                                 rsort_stream_t stream) {
+    if (ncaches > RSORT_MAX_CACHES)
+        return fail(RSORT_BAD_ARGUMENT, "cache count", RSORT_MAX_CACHES, ncaches);
+    rsort_status st = check_grid(batch, heads, capacity);
+    if (st != RSORT_OK) return st;
+    if (budget > size_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "cache budget");
+    if (ncaches == 0 || batch == 0 || heads == 0 || budget == 0 || capacity == 0) return RSORT_OK;
+    if (!caches || !d_kept || !d_kept_lengths) return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    st = check_alignment(addr(d_kept) | addr(d_kept_lengths), 4, "cache selection alignment");
+    if (st != RSORT_OK) return st;
+    const size_t bh = batch * heads;
+    const ByteRange kept = rows_range(d_kept, bh * budget, 4, 4);
+    const ByteRange kept_n = rows_range(d_kept_lengths, batch, 4, 4);
+    Strided in[RSORT_MAX_CACHES], out[RSORT_MAX_CACHES];
+    bool in_place = false;
+    for (size_t i = 0; i < ncaches; ++i) {
+        const rsort_cache_rows &c = caches[i];
+        if (c.row_bytes == 0 || c.row_bytes > size_t(INT_MAX))
+            return fail(RSORT_BAD_ARGUMENT, "cache row bytes", 1, c.row_bytes);
+        if (!c.src || !c.dst) return fail(RSORT_BAD_ARGUMENT, "null buffer");
+        const bool same = c.src == c.dst;
+        if (i && same != in_place)
+            return fail(RSORT_BAD_ARGUMENT, "caches move all in place or all out of place");
+        in_place = same;
+        if (same && (c.src_stride_b != c.dst_stride_b || c.src_stride_h != c.dst_stride_h ||
+                     c.src_stride_s != c.dst_stride_s))
+            return fail(RSORT_BAD_ARGUMENT, "cache strides in place");
+        if (!strided(c.src, batch, heads, capacity, c.src_stride_b, c.src_stride_h, c.src_stride_s,
+                     c.row_bytes, &in[i]) ||
+            !strided(c.dst, batch, heads, same || budget > capacity ? capacity : budget,
+                     c.dst_stride_b, c.dst_stride_h, c.dst_stride_s, c.row_bytes, &out[i]))
+            return fail(RSORT_SIZE_OVERFLOW, "cache strides");
+        if (!items_apart(out[i])) return fail(RSORT_BAD_ARGUMENT, "cache strides overlap");
+        if (overlap(out[i].range, kept) || overlap(out[i].range, kept_n))
+            return fail(RSORT_BAD_ARGUMENT, "caches overlap the kept positions");
+    }
+    for (size_t i = 0; i < ncaches; ++i)
+        for (size_t j = 0; j < ncaches; ++j)
+            if ((i != j && !arrays_apart(out[i], out[j])) ||
+                ((i != j || !in_place) && !arrays_apart(out[i], in[j])))
+                return fail(RSORT_BAD_ARGUMENT, "caches overlap");
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+
+    MoveArgs a{};
+    a.count = uint32_t(ncaches);
+    a.batch = uint32_t(batch);
+    a.heads = uint32_t(heads);
+    a.budget = uint32_t(budget);
+    a.capacity = uint32_t(capacity);
+    a.kept = d_kept;
+    a.kept_lengths = d_kept_lengths;
+    uint64_t blocks = 0;
+    for (size_t i = 0; i < ncaches; ++i) {
+        const rsort_cache_rows &c = caches[i];
+        Rows &r = a.rows[i];
+        r.src = static_cast<const char *>(c.src);
+        r.dst = static_cast<char *>(c.dst);
+        r.src_b = c.src_stride_b;
+        r.src_h = c.src_stride_h;
+        r.src_s = c.src_stride_s;
+        r.dst_b = c.dst_stride_b;
+        r.dst_h = c.dst_stride_h;
+        r.dst_s = c.dst_stride_s;
+        r.access = uint32_t(access_bytes(addr(c.src) | addr(c.dst) | r.src_b | r.src_h | r.src_s |
+                                             r.dst_b | r.dst_h | r.dst_s | c.row_bytes,
+                                         16));
+        r.units = uint32_t(c.row_bytes / r.access);
+        r.first_block = uint32_t(blocks);
+        if (in_place) {
+            // Slices of at least 64 bytes.
+            r.slices = uint32_t((c.row_bytes + 63) / 64);
+            blocks += r.slices;
+        } else {
+            const uint64_t per = MOVE_BLOCK * MOVE_STEPS;
+            blocks += (uint64_t(budget) * r.units + per - 1) / per;
+        }
+        if (blocks > uint64_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "cache rows");
+    }
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    LaunchScope scope(RSORT_KERNEL_CACHE, s);
+    const dim3 grid{unsigned(blocks), unsigned(bh)};
+    if (in_place)
+        cache_move_in_place_kernel<<<grid, MOVE_BLOCK, 0, s>>>(a);
+    else
+        cache_move_kernel<<<grid, MOVE_BLOCK, 0, s>>>(a);
+    return launched(cudaGetLastError(), "cache compaction launch");
+}
+
+}  // extern "C"

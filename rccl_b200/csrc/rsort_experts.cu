@@ -1,0 +1,620 @@
+// Expert routing: token slots sorted by expert, rows gathered into expert
+// order, expert outputs combined back with their weights, and the gradients.
+//
+// Slot s = token * top_k + k holds an expert id; ids outside 0..experts-1 are
+// dropped.  The sort is a stable counting sort: slot s of expert e goes to row
+// offsets[e] + (number of earlier slots of e), with every expert's segment
+// padded to a multiple of `align` rows.  The plan stays on the device.
+#include <climits>
+
+#include "../../include/rsort_b200.h"
+#include "rsort_internal.cuh"
+#include "rsort_rows.cuh"
+
+using namespace rsort;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Counting sort of slots by expert
+// ---------------------------------------------------------------------------
+constexpr int SORT_WARPS = 8;
+constexpr int SORT_BLOCK = SORT_WARPS * 32;
+
+struct SortArgs {
+    const void *ids;
+    uint32_t n;        // slots
+    uint32_t experts;
+    uint32_t align;
+    uint32_t chunk;    // slots per CTA, a multiple of SORT_BLOCK
+    uint32_t *counts_of_block;  // [grid][experts]
+    int32_t *row_of_slot, *slot_of_row;
+    uint32_t rows;     // capacity of slot_of_row
+    int32_t *offsets, *counts;
+};
+
+// The slot's bucket: its expert, or `experts` for a dropped slot.
+template <typename I>
+__device__ __forceinline__ uint32_t bucket(const SortArgs &a, uint32_t i) {
+    const I id = static_cast<const I *>(a.ids)[i];
+    return id >= 0 && id < I(a.experts) ? uint32_t(id) : a.experts;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(SORT_BLOCK) expert_count_kernel(const SortArgs a) {
+    extern __shared__ uint32_t hist[];  // experts + 1
+    for (uint32_t e = threadIdx.x; e <= a.experts; e += SORT_BLOCK) hist[e] = 0;
+    __syncthreads();
+    const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
+    const uint64_t last = min(first + a.chunk, uint64_t(a.n));
+    for (uint64_t i = first + threadIdx.x; i < last; i += SORT_BLOCK)
+        atomicAdd(&hist[bucket<I>(a, uint32_t(i))], 1u);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.experts; e += SORT_BLOCK)
+        a.counts_of_block[size_t(blockIdx.x) * a.experts + e] = hist[e];
+}
+
+template <typename I>
+__global__ void __launch_bounds__(SORT_BLOCK) expert_place_kernel(const SortArgs a) {
+    extern __shared__ uint32_t shared[];
+    const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t *const base = shared;                  // [SORT_WARPS][E + 1]
+    uint32_t *const start = base + SORT_WARPS * (E + 1);  // [E + 1] padded offsets
+    uint32_t *const total = start + E + 1;          // [E]
+    __shared__ uint32_t warp_sums[SORT_WARPS];
+    for (uint32_t i = tid; i < SORT_WARPS * (E + 1); i += SORT_BLOCK) base[i] = 0;
+    __syncthreads();
+
+    // Counts of this CTA's warps; each warp owns consecutive slots.
+    const uint64_t first = uint64_t(blockIdx.x) * a.chunk + uint64_t(warp) * (a.chunk / SORT_WARPS);
+    const uint64_t last = min(first + a.chunk / SORT_WARPS, uint64_t(a.n));
+    uint32_t *const mine = base + warp * (E + 1);
+    for (uint64_t i = first + lane; i < last; i += 32)
+        atomicAdd(&mine[bucket<I>(a, uint32_t(i))], 1u);
+    __syncthreads();
+
+    // Totals over all CTAs and the part of the earlier ones, then the warps'
+    // running counts inside this CTA.
+    for (uint32_t e = tid; e < E; e += SORT_BLOCK) {
+        uint32_t before = 0, all = 0;
+        for (uint32_t c = 0; c < gridDim.x; ++c) {
+            const uint32_t v = a.counts_of_block[size_t(c) * E + e];
+            if (c < blockIdx.x) before += v;
+            all += v;
+        }
+        total[e] = all;
+        for (uint32_t w = 0; w < SORT_WARPS; ++w) {
+            const uint32_t v = base[w * (E + 1) + e];
+            base[w * (E + 1) + e] = before;
+            before += v;
+        }
+    }
+    __syncthreads();
+
+    // Exclusive scan of the padded segment sizes, SORT_BLOCK experts a step.
+    uint32_t carry = 0;
+    for (uint32_t e0 = 0; e0 < E; e0 += SORT_BLOCK) {
+        const uint32_t e = e0 + tid;
+        const uint32_t size = e < E ? (total[e] + a.align - 1) / a.align * a.align : 0;
+        uint32_t inc = size;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
+            if (lane >= uint32_t(off)) inc += y;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
+        __syncthreads();
+        uint32_t sum = carry;
+        for (uint32_t w = 0; w < SORT_WARPS; ++w) {
+            if (w == warp && e < E) start[e] = sum + inc - size;
+            sum += warp_sums[w];
+        }
+        carry = sum;
+        __syncthreads();
+    }
+    if (tid == 0) start[E] = carry;
+    __syncthreads();
+
+    // Rows of this warp's slots: lanes with the same expert take consecutive
+    // rows in lane order, so the order of the slots is kept.
+    for (uint64_t i0 = first; i0 < last; i0 += 32) {
+        const uint64_t i = i0 + lane;
+        const bool in = i < last;
+        const uint32_t e = in ? bucket<I>(a, uint32_t(i)) : E;
+        const uint32_t peers = __match_any_sync(0xffffffffu, e);
+        const uint32_t rank = __popc(peers & ((1u << lane) - 1));
+        const uint32_t at = mine[e];
+        __syncwarp();
+        if (rank == 0) mine[e] = at + __popc(peers);
+        __syncwarp();
+        if (in) {
+            int32_t row = -1;
+            if (e < E) {
+                row = int32_t(start[e] + at + rank);
+                if (uint32_t(row) < a.rows) a.slot_of_row[row] = int32_t(i);
+            }
+            a.row_of_slot[i] = row;
+        }
+    }
+
+    // Padding rows of the experts, the rows behind the last segment, and the
+    // segments themselves.
+    for (uint32_t e = blockIdx.x; e <= E; e += gridDim.x) {
+        const uint32_t lo = e < E ? start[e] + total[e] : start[E];
+        const uint32_t hi = e < E ? start[e + 1] : a.rows;
+        for (uint32_t r = lo + tid; r < hi && r < a.rows; r += SORT_BLOCK) a.slot_of_row[r] = -1;
+    }
+    if (blockIdx.x == 0) {
+        for (uint32_t e = tid; e <= E; e += SORT_BLOCK) {
+            a.offsets[e] = int32_t(start[e]);
+            if (e < E) a.counts[e] = int32_t(total[e]);
+        }
+    }
+}
+
+uint32_t sort_grid(size_t n, int sm_count) {
+    const size_t want = (n + 1023) / 1024;
+    return uint32_t(want < 1 ? 1 : want < size_t(sm_count) ? want : size_t(sm_count));
+}
+
+constexpr int SORT_MAX_GRID = 1024;  // scratch is sized for this many CTAs
+
+// ---------------------------------------------------------------------------
+// Rows in and out of expert order
+// ---------------------------------------------------------------------------
+constexpr int ROW_BLOCK = 256;
+constexpr int PAD_BLOCKS = 4;  // CTAs that zero one expert's padding rows
+
+struct Plan {
+    const int32_t *row_of_slot, *offsets, *counts;
+    uint32_t tokens, top_k, experts, rows;
+};
+
+// `lanes` threads (a power of two up to ROW_BLOCK) work on one token.
+struct Shape {
+    uint32_t lanes, token_blocks, units;
+};
+
+Shape shape_of(size_t tokens, size_t units) {
+    Shape s{1, 0, uint32_t(units)};
+    while (s.lanes < ROW_BLOCK && s.lanes < units) s.lanes <<= 1;
+    const uint32_t per = ROW_BLOCK / s.lanes;
+    s.token_blocks = uint32_t((tokens + per - 1) / per);
+    return s;
+}
+
+// A slot's row, or -1 when it was dropped (or the plan does not fit the rows).
+__device__ __forceinline__ int32_t row_at(const Plan &p, uint64_t slot) {
+    const int32_t r = p.row_of_slot[slot];
+    return uint32_t(r) < p.rows ? r : -1;
+}
+
+// Zeros the padding rows of one expert (block b of the padding blocks).
+template <typename U>
+__device__ __forceinline__ void zero_padding(const Plan &p, uint32_t b, char *rows, size_t stride,
+                                             uint32_t units) {
+    const uint32_t e = b / PAD_BLOCKS;
+    const uint32_t lo = uint32_t(p.offsets[e]) + uint32_t(p.counts[e]);
+    const uint32_t hi = min(uint32_t(p.offsets[e + 1]), p.rows);
+    for (uint32_t r = lo + b % PAD_BLOCKS; r < hi; r += PAD_BLOCKS) {
+        U *row = reinterpret_cast<U *>(rows + size_t(r) * stride);
+        for (uint32_t u = threadIdx.x; u < units; u += ROW_BLOCK) row[u] = U{};
+    }
+}
+
+template <typename U>
+__global__ void __launch_bounds__(ROW_BLOCK)
+    expert_gather_kernel(const Plan p, const Shape s, const char *x, size_t x_stride, char *rows,
+                         size_t rows_stride) {
+    if (blockIdx.x >= s.token_blocks) {
+        zero_padding<U>(p, blockIdx.x - s.token_blocks, rows, rows_stride, s.units);
+        return;
+    }
+    const uint32_t t = blockIdx.x * (ROW_BLOCK / s.lanes) + threadIdx.x / s.lanes;
+    if (t >= p.tokens) return;
+    const U *src = reinterpret_cast<const U *>(x + size_t(t) * x_stride);
+    for (uint32_t u = threadIdx.x % s.lanes; u < s.units; u += s.lanes) {
+        const U v = src[u];
+        for (uint32_t k = 0; k < p.top_k; ++k) {
+            const int32_t r = row_at(p, uint64_t(t) * p.top_k + k);
+            if (r >= 0) reinterpret_cast<U *>(rows + size_t(r) * rows_stride)[u] = v;
+        }
+    }
+}
+
+struct Weights {
+    const void *w;  // null: every weight is 1
+    int type;       // rsort_key_t
+};
+
+__device__ __forceinline__ float weight_at(const Weights &w, uint64_t slot) {
+    if (!w.w) return 1.0f;
+    if (w.type == RSORT_F32) return static_cast<const float *>(w.w)[slot];
+    if (w.type == RSORT_F16) return __half2float(static_cast<const __half *>(w.w)[slot]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(w.w)[slot]);
+}
+
+__device__ __forceinline__ void store_weight(void *w, int type, uint64_t slot, float v) {
+    if (type == RSORT_F32) static_cast<float *>(w)[slot] = v;
+    else if (type == RSORT_F16) static_cast<__half *>(w)[slot] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(w)[slot] = __float2bfloat16_rn(v);
+}
+
+// out[t] = sum over k of weight * rows[row of slot], summed in fp32 in the
+// order of k and rounded once.
+template <typename T, int V>
+__global__ void __launch_bounds__(ROW_BLOCK)
+    expert_combine_kernel(const Plan p, const Shape s, const T *rows, size_t rows_stride,
+                          const Weights w, T *out, size_t out_stride) {
+    const uint32_t t = blockIdx.x * (ROW_BLOCK / s.lanes) + threadIdx.x / s.lanes;
+    if (t >= p.tokens) return;
+    using P = Pack<T, V>;
+    P *dst = reinterpret_cast<P *>(out + size_t(t) * out_stride);
+    for (uint32_t u = threadIdx.x % s.lanes; u < s.units; u += s.lanes) {
+        float acc[V] = {};
+#pragma unroll 4
+        for (uint32_t k = 0; k < p.top_k; ++k) {
+            const uint64_t slot = uint64_t(t) * p.top_k + k;
+            const int32_t r = row_at(p, slot);
+            if (r < 0) continue;
+            const P v = reinterpret_cast<const P *>(rows + size_t(r) * rows_stride)[u];
+            const float f = weight_at(w, slot);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(f, to_float(v.v[i]), acc[i]);
+        }
+        P o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(acc[i]);
+        dst[u] = o;
+    }
+}
+
+// grad_rows[row of slot] = weight * grad_out[t], grad_w[slot] = the dot
+// product of grad_out[t] and rows[row of slot] in fp32; DOT_K slots a pass.
+constexpr int DOT_K = 8;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(ROW_BLOCK)
+    expert_combine_backward_kernel(const Plan p, const Shape s, const T *grad_out,
+                                   size_t grad_out_stride, const T *rows, size_t rows_stride,
+                                   const Weights w, T *grad_rows, size_t grad_rows_stride,
+                                   void *grad_w) {
+    using P = Pack<T, V>;
+    if (blockIdx.x >= s.token_blocks) {
+        zero_padding<P>(p, blockIdx.x - s.token_blocks, reinterpret_cast<char *>(grad_rows),
+                        grad_rows_stride * sizeof(T), s.units);
+        return;
+    }
+    __shared__ float sums[ROW_BLOCK / 32][DOT_K];
+    const uint32_t t = blockIdx.x * (ROW_BLOCK / s.lanes) + threadIdx.x / s.lanes;
+    const uint32_t lane0 = threadIdx.x % s.lanes;
+    const bool live = t < p.tokens;
+    const P *g = reinterpret_cast<const P *>(grad_out + size_t(live ? t : 0) * grad_out_stride);
+    for (uint32_t k0 = 0; k0 < p.top_k; k0 += DOT_K) {
+        float dot[DOT_K] = {};
+        const uint32_t nk = min(uint32_t(DOT_K), p.top_k - k0);
+        const uint64_t slot0 = uint64_t(t) * p.top_k + k0;
+        if (live) {
+            for (uint32_t u = lane0; u < s.units; u += s.lanes) {
+                const P gv = g[u];
+#pragma unroll
+                for (int k = 0; k < DOT_K; ++k) {
+                    const int32_t r = uint32_t(k) < nk ? row_at(p, slot0 + k) : -1;
+                    if (r < 0) continue;
+                    if (grad_w) {
+                        const P v = reinterpret_cast<const P *>(rows + size_t(r) * rows_stride)[u];
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            dot[k] = fmaf(to_float(gv.v[i]), to_float(v.v[i]), dot[k]);
+                    }
+                    if (grad_rows) {
+                        const float f = weight_at(w, slot0 + k);
+                        P o;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(f * to_float(gv.v[i]));
+                        reinterpret_cast<P *>(grad_rows + size_t(r) * grad_rows_stride)[u] = o;
+                    }
+                }
+            }
+        }
+        if (!grad_w) continue;
+        // Sum over the token's threads: lanes of a warp first, then warps.
+        const uint32_t width = min(s.lanes, 32u);
+#pragma unroll
+        for (int k = 0; k < DOT_K; ++k)
+            for (uint32_t o = width / 2; o > 0; o >>= 1)
+                dot[k] += __shfl_down_sync(0xffffffffu, dot[k], o, width);
+        if (s.lanes <= 32) {
+            if (live && lane0 == 0)
+                for (int k = 0; k < DOT_K; ++k)
+                    if (uint32_t(k) < nk) store_weight(grad_w, w.type, slot0 + k, dot[k]);
+            continue;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int k = 0; k < DOT_K; ++k) sums[threadIdx.x >> 5][k] = dot[k];
+        __syncthreads();
+        if (live && lane0 < nk) {
+            float total = 0;
+            const uint32_t w0 = threadIdx.x / s.lanes * (s.lanes / 32);
+            for (uint32_t i = 0; i < s.lanes / 32; ++i) total += sums[w0 + i][lane0];
+            store_weight(grad_w, w.type, slot0 + lane0, total);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Argument checks
+// ---------------------------------------------------------------------------
+size_t rows_bound(size_t nslots, size_t experts, size_t align) {
+    const size_t used = experts < nslots ? experts : nslots;
+    return (nslots + used * (align - 1)) / align * align;
+}
+
+bool sort_shape_ok(size_t nslots, size_t experts, size_t align) {
+    return experts >= 1 && experts <= RSORT_MAX_EXPERTS && align >= 1 &&
+           align <= RSORT_MAX_EXPERT_ALIGN && nslots <= size_t(INT_MAX) &&
+           rows_bound(nslots, experts, align) <= size_t(INT_MAX);
+}
+
+rsort_status check_plan(const rsort_expert_plan *p, Plan *out) {
+    if (!p) return fail(RSORT_BAD_ARGUMENT, "null expert plan");
+    if (p->experts < 1 || p->experts > RSORT_MAX_EXPERTS)
+        return fail(RSORT_BAD_ARGUMENT, "expert count", RSORT_MAX_EXPERTS, p->experts);
+    if (p->top_k < 1) return fail(RSORT_BAD_ARGUMENT, "expert plan top_k");
+    if (p->tokens > size_t(INT_MAX) / p->top_k || p->nrows > size_t(INT_MAX))
+        return fail(RSORT_SIZE_OVERFLOW, "expert plan (32-bit slots and rows)");
+    if (!p->offsets || !p->counts || (p->tokens && !p->row_of_slot))
+        return fail(RSORT_BAD_ARGUMENT, "null expert plan array");
+    if (check_alignment(addr(p->offsets) | addr(p->counts) | addr(p->row_of_slot), 4,
+                        "expert plan alignment") != RSORT_OK)
+        return RSORT_BAD_ARGUMENT;
+    *out = Plan{p->row_of_slot, p->offsets, p->counts, uint32_t(p->tokens), uint32_t(p->top_k),
+                uint32_t(p->experts), uint32_t(p->nrows)};
+    return RSORT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rsort_expert_rows(size_t nslots, size_t experts, size_t align) {
+    return sort_shape_ok(nslots, experts, align) ? rows_bound(nslots, experts, align) : 0;
+}
+
+size_t rsort_expert_sort_scratch_bytes(size_t nslots, size_t experts) {
+    if (experts < 1 || experts > RSORT_MAX_EXPERTS || nslots > size_t(INT_MAX)) return 0;
+    return sort_grid(nslots, SORT_MAX_GRID) * experts * sizeof(uint32_t);
+}
+
+rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t nslots,
+                               size_t experts, size_t align, int32_t *d_row_of_slot,
+                               int32_t *d_slot_of_row, size_t nrows, int32_t *d_offsets,
+                               int32_t *d_counts, void *d_scratch, size_t scratch_bytes,
+                               rsort_stream_t stream) {
+    if (id_type != RSORT_I32 && id_type != RSORT_I64)
+        return fail(RSORT_BAD_ARGUMENT, "expert id type (i32 or i64)");
+    if (experts < 1 || experts > RSORT_MAX_EXPERTS)
+        return fail(RSORT_BAD_ARGUMENT, "expert count", RSORT_MAX_EXPERTS, experts);
+    if (align < 1 || align > RSORT_MAX_EXPERT_ALIGN)
+        return fail(RSORT_BAD_ARGUMENT, "expert alignment", RSORT_MAX_EXPERT_ALIGN, align);
+    if (!sort_shape_ok(nslots, experts, align) || nrows > size_t(INT_MAX))
+        return fail(RSORT_SIZE_OVERFLOW, "expert rows (32-bit slots and rows)");
+    const size_t need = rows_bound(nslots, experts, align);
+    if (nrows < need) return fail(RSORT_WORKSPACE_TOO_SMALL, "expert rows", need, nrows);
+    if ((nslots && (!d_ids || !d_row_of_slot)) || (nrows && !d_slot_of_row) || !d_offsets ||
+        !d_counts)
+        return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    const size_t bytes = rsort_expert_sort_scratch_bytes(nslots, experts);
+    if (!d_scratch || scratch_bytes < bytes)
+        return fail(RSORT_WORKSPACE_TOO_SMALL, "expert sort scratch", bytes, scratch_bytes);
+    rsort_status st = check_alignment(addr(d_ids), id_type == RSORT_I64 ? 8 : 4,
+                                      "expert ids alignment");
+    if (st == RSORT_OK)
+        st = check_alignment(addr(d_row_of_slot) | addr(d_slot_of_row) | addr(d_offsets) |
+                                 addr(d_counts) | addr(d_scratch),
+                             4, "expert plan alignment");
+    if (st != RSORT_OK) return st;
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    if (sms > SORT_MAX_GRID) sms = SORT_MAX_GRID;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+
+    SortArgs a{};
+    a.ids = d_ids;
+    a.n = uint32_t(nslots);
+    a.experts = uint32_t(experts);
+    a.align = uint32_t(align);
+    const uint32_t grid = sort_grid(nslots, sms);
+    a.chunk = uint32_t(((nslots + grid - 1) / grid + SORT_BLOCK - 1) / SORT_BLOCK * SORT_BLOCK);
+    a.counts_of_block = static_cast<uint32_t *>(d_scratch);
+    a.row_of_slot = d_row_of_slot;
+    a.slot_of_row = d_slot_of_row;
+    a.rows = uint32_t(nrows);
+    a.offsets = d_offsets;
+    a.counts = d_counts;
+    const size_t count_shared = (experts + 1) * 4;
+    const size_t place_shared = (SORT_WARPS * (experts + 1) + 2 * experts + 1) * 4;
+    {
+        LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
+        if (id_type == RSORT_I32)
+            expert_count_kernel<int32_t><<<grid, SORT_BLOCK, count_shared, s>>>(a);
+        else
+            expert_count_kernel<int64_t><<<grid, SORT_BLOCK, count_shared, s>>>(a);
+    }
+    {
+        LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
+        if (id_type == RSORT_I32)
+            expert_place_kernel<int32_t><<<grid, SORT_BLOCK, place_shared, s>>>(a);
+        else
+            expert_place_kernel<int64_t><<<grid, SORT_BLOCK, place_shared, s>>>(a);
+    }
+    return launched(cudaGetLastError(), "expert sort launch");
+}
+
+rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x, size_t x_stride,
+                                 void *d_rows, size_t rows_stride, size_t row_bytes,
+                                 int zero_padding_rows, rsort_stream_t stream) {
+    Plan p{};
+    rsort_status st = check_plan(plan, &p);
+    if (st != RSORT_OK) return st;
+    if (row_bytes > size_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "expert row bytes");
+    if (row_bytes == 0 || p.rows == 0) return RSORT_OK;
+    if ((p.tokens && !d_x) || !d_rows) return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    if (p.rows > 1 && rows_stride < row_bytes)
+        return fail(RSORT_BAD_ARGUMENT, "expert rows stride", row_bytes, rows_stride);
+    if (!rows_fit(p.tokens, x_stride, row_bytes) || !rows_fit(p.rows, rows_stride, row_bytes))
+        return fail(RSORT_SIZE_OVERFLOW, "expert rows");
+    if (overlap(rows_range(d_x, p.tokens, x_stride, row_bytes),
+                rows_range(d_rows, p.rows, rows_stride, row_bytes)))
+        return fail(RSORT_BAD_ARGUMENT, "expert rows overlap the tokens");
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const size_t access =
+        access_bytes(addr(d_x) | addr(d_rows) | x_stride | rows_stride | row_bytes, 16);
+    const Shape shape = shape_of(p.tokens, row_bytes / access);
+    const uint32_t grid = shape.token_blocks + (zero_padding_rows ? p.experts * PAD_BLOCKS : 0);
+    if (grid == 0) return RSORT_OK;
+    auto go = [&](auto unit) {
+        expert_gather_kernel<decltype(unit)><<<grid, ROW_BLOCK, 0, s>>>(
+            p, shape, static_cast<const char *>(d_x), x_stride, static_cast<char *>(d_rows),
+            rows_stride);
+        return cudaGetLastError();
+    };
+    LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
+    return launched(access == 16  ? go(uint4{})
+                    : access == 8 ? go(uint2{})
+                    : access == 4 ? go(uint32_t{})
+                    : access == 2 ? go(uint16_t{})
+                                  : go(uint8_t{}),
+                    "expert gather launch");
+}
+
+rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t type,
+                                  const void *d_rows, size_t rows_stride, const void *d_weights,
+                                  rsort_key_t weight_type, void *d_out, size_t out_stride,
+                                  size_t width, rsort_stream_t stream) {
+    Plan p{};
+    rsort_status st = check_plan(plan, &p);
+    if (st != RSORT_OK) return st;
+    const size_t eb = real_bytes(type);
+    if (!eb) return fail(RSORT_BAD_ARGUMENT, "expert row type (f32, f16 or bf16)");
+    if (d_weights && !real_bytes(weight_type))
+        return fail(RSORT_BAD_ARGUMENT, "expert weight type (f32, f16 or bf16)");
+    if (width > size_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "expert row width");
+    if (width == 0 || p.tokens == 0) return RSORT_OK;
+    if ((p.rows && !d_rows) || !d_out) return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    if (p.tokens > 1 && out_stride < width)
+        return fail(RSORT_BAD_ARGUMENT, "expert output stride", width, out_stride);
+    constexpr size_t most = size_t(1) << 53;
+    if (rows_stride > most || out_stride > most || !rows_fit(p.rows, rows_stride * eb, width * eb) ||
+        !rows_fit(p.tokens, out_stride * eb, width * eb))
+        return fail(RSORT_SIZE_OVERFLOW, "expert rows");
+    st = check_alignment(addr(d_rows) | addr(d_out), eb, "expert rows alignment");
+    if (st == RSORT_OK && d_weights)
+        st = check_alignment(addr(d_weights), real_bytes(weight_type), "expert weights alignment");
+    if (st != RSORT_OK) return st;
+    const ByteRange out = rows_range(d_out, p.tokens, out_stride * eb, width * eb);
+    if (overlap(rows_range(d_rows, p.rows, rows_stride * eb, width * eb), out))
+        return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the rows");
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const size_t access = access_bytes(
+        addr(d_rows) | addr(d_out) | rows_stride * eb | out_stride * eb | width * eb, 16);
+    const Weights w{d_weights, int(weight_type)};
+    LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
+    return launched(with_type(type, access,
+                              [&](auto t, auto v) {
+                                  using T = decltype(t);
+                                  constexpr int V = decltype(v)::value;
+                                  const Shape shape = shape_of(p.tokens, width / V);
+                                  expert_combine_kernel<T, V>
+                                      <<<shape.token_blocks, ROW_BLOCK, 0, s>>>(
+                                          p, shape, static_cast<const T *>(d_rows), rows_stride, w,
+                                          static_cast<T *>(d_out), out_stride);
+                                  return cudaGetLastError();
+                              }),
+                    "expert combine launch");
+}
+
+rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_key_t type,
+                                           const void *d_grad_out, size_t grad_out_stride,
+                                           const void *d_rows, size_t rows_stride,
+                                           const void *d_weights, rsort_key_t weight_type,
+                                           void *d_grad_rows, size_t grad_rows_stride,
+                                           void *d_grad_weights, size_t width,
+                                           int zero_padding_rows, rsort_stream_t stream) {
+    Plan p{};
+    rsort_status st = check_plan(plan, &p);
+    if (st != RSORT_OK) return st;
+    const size_t eb = real_bytes(type);
+    if (!eb) return fail(RSORT_BAD_ARGUMENT, "expert row type (f32, f16 or bf16)");
+    const size_t wb = real_bytes(weight_type);
+    if (!wb) return fail(RSORT_BAD_ARGUMENT, "expert weight type (f32, f16 or bf16)");
+    if (width > size_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "expert row width");
+    if (!d_grad_rows && !d_grad_weights)
+        return fail(RSORT_BAD_ARGUMENT, "expert combine gradient without an output");
+    if (p.tokens && width && (!d_grad_out || (d_grad_weights && p.rows && !d_rows)))
+        return fail(RSORT_BAD_ARGUMENT, "null buffer");
+    if (d_grad_rows && p.rows > 1 && grad_rows_stride < width)
+        return fail(RSORT_BAD_ARGUMENT, "expert gradient rows stride", width, grad_rows_stride);
+    constexpr size_t most = size_t(1) << 53;
+    if (rows_stride > most || grad_out_stride > most || grad_rows_stride > most ||
+        !rows_fit(p.rows, rows_stride * eb, width * eb) ||
+        !rows_fit(p.rows, grad_rows_stride * eb, width * eb) ||
+        !rows_fit(p.tokens, grad_out_stride * eb, width * eb))
+        return fail(RSORT_SIZE_OVERFLOW, "expert rows");
+    st = check_alignment(addr(d_grad_out) | addr(d_rows) | addr(d_grad_rows), eb,
+                         "expert rows alignment");
+    if (st == RSORT_OK)
+        st = check_alignment(addr(d_weights) | addr(d_grad_weights), wb,
+                             "expert weights alignment");
+    if (st != RSORT_OK) return st;
+    if (d_grad_rows) {
+        const ByteRange out =
+            rows_range(d_grad_rows, p.rows, grad_rows_stride * eb, width * eb);
+        if (overlap(out, rows_range(d_grad_out, p.tokens, grad_out_stride * eb, width * eb)) ||
+            (d_grad_weights && d_rows &&
+             overlap(out, rows_range(d_rows, p.rows, rows_stride * eb, width * eb))))
+            return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
+    }
+    const size_t slots = size_t(p.tokens) * p.top_k;
+    if (d_grad_weights && d_weights &&
+        overlap(rows_range(d_grad_weights, slots, wb, wb), rows_range(d_weights, slots, wb, wb)))
+        return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap the weights");
+    int sms = 0;
+    st = current_sm_count(&sms);
+    if (st != RSORT_OK) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    size_t bits = addr(d_grad_out) | grad_out_stride * eb | width * eb;
+    if (d_grad_weights) bits |= addr(d_rows) | rows_stride * eb;
+    if (d_grad_rows) bits |= addr(d_grad_rows) | grad_rows_stride * eb;
+    const size_t access = access_bytes(bits, 16);
+    const Weights w{d_weights, int(weight_type)};
+    LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
+    return launched(
+        with_type(type, access,
+                  [&](auto t, auto v) {
+                      using T = decltype(t);
+                      constexpr int V = decltype(v)::value;
+                      const Shape shape = shape_of(p.tokens, width / V);
+                      const uint32_t grid =
+                          shape.token_blocks +
+                          (zero_padding_rows && d_grad_rows ? p.experts * PAD_BLOCKS : 0);
+                      if (grid == 0) return cudaSuccess;
+                      expert_combine_backward_kernel<T, V><<<grid, ROW_BLOCK, 0, s>>>(
+                          p, shape, static_cast<const T *>(d_grad_out), grad_out_stride,
+                          static_cast<const T *>(d_rows), rows_stride, w,
+                          static_cast<T *>(d_grad_rows), grad_rows_stride, d_grad_weights);
+                      return cudaGetLastError();
+                  }),
+        "expert combine gradient launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,92 @@
+// Shared by the operators that move wide rows (expert routing and cache
+// eviction): the element types they compute in, packs of elements moved with
+// one access, and the argument checks of strided row ranges.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "rsort_internal.cuh"
+
+namespace rsort {
+
+// V elements moved with one access; the address is aligned to the pack.
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) {
+    return __float2half_rn(x);
+}
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+
+// The types that rows with arithmetic may have, and their sizes (0: not one).
+inline size_t real_bytes(rsort_key_t t) {
+    return t == RSORT_F32 ? 4 : (t == RSORT_F16 || t == RSORT_BF16) ? 2 : 0;
+}
+
+// Largest power of two (at most `most`) that divides every address and
+// stride OR-ed into `bits`: the widest access the rows allow.
+inline size_t access_bytes(uintptr_t bits, size_t most) {
+    size_t a = most;
+    while (a > 1 && (bits & (a - 1)) != 0) a >>= 1;
+    return a;
+}
+
+// [first, last) of n rows of `bytes`, `stride` bytes apart.
+struct ByteRange {
+    uintptr_t first, last;
+};
+inline ByteRange rows_range(const void *p, size_t n, size_t stride, size_t bytes) {
+    if (n == 0 || bytes == 0) return {addr(p), addr(p)};
+    return {addr(p), addr(p) + (n - 1) * stride + bytes};
+}
+inline bool overlap(const ByteRange &a, const ByteRange &b) {
+    return a.first < a.last && b.first < b.last && a.first < b.last && b.first < a.last;
+}
+
+// n rows `stride` bytes apart stay below 2^56 bytes, far beyond any device,
+// so no offset of theirs wraps.
+inline bool rows_fit(size_t n, size_t stride, size_t bytes) {
+    constexpr size_t kMost = size_t(1) << 56;
+    return bytes <= kMost && (n == 0 || stride <= kMost / n);
+}
+
+inline rsort_status fail(rsort_status s, const char *role, size_t expected = 0,
+                         size_t actual = 0) {
+    return record_failure(s, role, expected, actual);
+}
+
+inline rsort_status launched(cudaError_t e, const char *role) {
+    return e == cudaSuccess ? RSORT_OK : fail(RSORT_CUDA_ERROR, role);
+}
+
+// Calls f with the element type and the elements of one access.
+template <typename F> cudaError_t with_type(rsort_key_t type, size_t access, F f) {
+    if (type == RSORT_F32) {
+        if (access >= 16) return f(float{}, std::integral_constant<int, 4>{});
+        if (access >= 8) return f(float{}, std::integral_constant<int, 2>{});
+        return f(float{}, std::integral_constant<int, 1>{});
+    }
+    auto half = [&](auto t) {
+        if (access >= 16) return f(t, std::integral_constant<int, 8>{});
+        if (access >= 8) return f(t, std::integral_constant<int, 4>{});
+        if (access >= 4) return f(t, std::integral_constant<int, 2>{});
+        return f(t, std::integral_constant<int, 1>{});
+    };
+    return type == RSORT_F16 ? half(__half{}) : half(__nv_bfloat16{});
+}
+
+}  // namespace rsort

@@ -1,0 +1,159 @@
+"""Cache eviction by accumulated attention weight (no reference counterpart).
+
+The segmented selection and compaction that a key/value cache of bounded size
+needs, beside the segmented sort.  A serving loop calls, on one launch:
+
+    device_attention_weight_add(launch, weights, scores, lengths)   # every step
+    device_cache_select(launch, scores, lengths, kept, kept_lengths,
+                        sinks=4, recent=64)                         # when full
+    device_cache_compact(launch, kept, kept_lengths, [k, v, scores])  # in place
+
+scores (batch, heads, capacity) float32 totals; lengths (batch,) int32
+positions in use; kept (batch, heads, budget) int32.  All memory is the
+caller's, every call is asynchronous on the launch's stream and reads nothing
+back, so a step can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from .cub import Launch
+from .errors import BadArgument, LengthMismatch
+from .experts import _on, call, real_code
+
+
+def _int32(role: str, t: torch.Tensor, *shape: int) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise BadArgument(f"{role} must be contiguous int32")
+    if tuple(t.shape) != shape:
+        raise LengthMismatch(role, _count(shape), t.numel())
+
+
+def _count(shape) -> int:
+    n = 1
+    for s in shape:
+        n *= s
+    return n
+
+
+def _scores(t: torch.Tensor) -> None:
+    if t.dtype != torch.float32 or t.dim() != 3 or (
+            t.numel() and t.shape[2] != 1 and t.stride(2) != 1):
+        raise BadArgument("cache scores must be (batch, heads, capacity) float32 with "
+                          "neighbouring positions")
+
+
+def device_attention_weight_add(launch: Launch, weights: torch.Tensor, scores: torch.Tensor,
+                                lengths: Optional[torch.Tensor] = None, decay: float = 1.0,
+                                causal: bool = False) -> None:
+    """scores[b, h, s] = decay * scores[b, h, s] + the attention weights that
+    position s got, summed in fp32 over the queries and over the query heads of
+    cache head h, for s < lengths[b] (every position without lengths).
+
+    weights (batch, query heads, queries, capacity), or (batch, query heads,
+    capacity) for a single token: float32, float16 or bfloat16; query head
+    h * group + g reads cache head h.  With causal the queries are the last
+    ones of each sequence and what a query does not see is not read."""
+    _on(launch, weights, scores, lengths)
+    if weights.dim() == 3:
+        weights = weights.unsqueeze(2)
+    code = real_code(weights.dtype)
+    _scores(scores)
+    batch, heads, capacity = scores.shape
+    if weights.dim() != 4 or (
+            weights.numel() and capacity != 1 and weights.stride(3) != 1):
+        raise BadArgument("attention weights must be (batch, query heads[, queries], capacity) "
+                          "with neighbouring positions")
+    if weights.shape[0] != batch:
+        raise LengthMismatch("attention weight batch", batch, weights.shape[0])
+    if weights.shape[3] != capacity:
+        raise LengthMismatch("attention weight positions", capacity, weights.shape[3])
+    group = weights.shape[1] // heads if heads else 1
+    if group * heads != weights.shape[1] or group < 1:
+        raise LengthMismatch("attention weight heads", max(group, 1) * heads, weights.shape[1])
+    if lengths is not None:
+        _int32("cache lengths", lengths, batch)
+    sb, sh, sq, _ = weights.stride()
+    call(launch, _lib.lib().rsort_attention_weight_add, code, weights.data_ptr(), sb, sh, sq,
+         batch, heads, group, weights.shape[2], capacity,
+         None if lengths is None else lengths.data_ptr(), decay, int(causal), scores.data_ptr(),
+         scores.stride(0), scores.stride(1))
+
+
+def device_cache_select(launch: Launch, scores: torch.Tensor, lengths: Optional[torch.Tensor],
+                        kept: torch.Tensor, kept_lengths: torch.Tensor, sinks: int = 0,
+                        recent: int = 0) -> None:
+    """The positions of every head that stay: kept (batch, heads, budget)
+    ascending, then -1; kept_lengths (batch,) = min(lengths, budget).  The first
+    `sinks`, the last `recent` and the heaviest between stay; equal totals keep
+    the lower position, NaN counts as -inf.  kept_lengths must not be lengths."""
+    _on(launch, scores, lengths, kept, kept_lengths)
+    _scores(scores)
+    batch, heads, capacity = scores.shape
+    if kept.dim() != 3:
+        raise BadArgument("kept positions must be (batch, heads, budget)")
+    budget = kept.shape[2]
+    _int32("kept positions", kept, batch, heads, budget)
+    _int32("kept lengths", kept_lengths, batch)
+    if lengths is not None:
+        _int32("cache lengths", lengths, batch)
+    if sinks < 0 or recent < 0:
+        raise BadArgument(f"{sinks} sinks, {recent} recent positions")
+    call(launch, _lib.lib().rsort_cache_select, scores.data_ptr(), scores.stride(0),
+         scores.stride(1), None if lengths is None else lengths.data_ptr(), batch, heads,
+         capacity, budget, sinks, recent, kept.data_ptr(), kept_lengths.data_ptr())
+
+
+def device_cache_compact(launch: Launch, kept: torch.Tensor, kept_lengths: torch.Tensor,
+                         sources: Sequence[torch.Tensor],
+                         destinations: Optional[Sequence[torch.Tensor]] = None) -> None:
+    """destinations[i][b, h, j] = sources[i][b, h, kept[b, h, j]] for
+    j < kept_lengths[b], all arrays in one launch; later rows are left as they
+    are.  Arrays are (batch, heads, capacity) or (batch, heads, capacity, width)
+    of any element type and any strides but neighbouring elements in a row
+    (pass a transposed view of a (batch, capacity, heads, width) cache).
+    Without destinations, or with the sources themselves, the cache is
+    compacted in place by ascending kept positions."""
+    if destinations is None:
+        destinations = sources
+    if len(sources) != len(destinations):
+        raise LengthMismatch("compacted caches", len(sources), len(destinations))
+    if len(sources) > _lib.MAX_CACHES:
+        raise BadArgument(f"{len(sources)} caches (at most {_lib.MAX_CACHES})")
+    _on(launch, kept, kept_lengths, *sources, *destinations)
+    if kept.dim() != 3:
+        raise BadArgument("kept positions must be (batch, heads, budget)")
+    batch, heads, budget = kept.shape
+    _int32("kept positions", kept, batch, heads, budget)
+    _int32("kept lengths", kept_lengths, batch)
+    capacity = sources[0].shape[2] if sources and sources[0].dim() >= 3 else 0
+    rows = (_lib.CacheRows * max(len(sources), 1))()
+    for r, src, dst in zip(rows, sources, destinations):
+        if src.dim() not in (3, 4) or dst.dim() != src.dim():
+            raise BadArgument("caches must be (batch, heads, capacity[, width])")
+        if dst.dtype != src.dtype:
+            raise BadArgument(f"cache of {src.dtype} into {dst.dtype}")
+        ss, ds = src.shape, dst.shape
+        if ss[0] != batch or ss[1] != heads or ss[2] != capacity:
+            raise LengthMismatch("cache", batch * heads * capacity, ss[0] * ss[1] * ss[2])
+        if ds[0] != batch or ds[1] != heads or ds[3:] != ss[3:]:
+            raise LengthMismatch("compacted cache", _count(ss[:2] + ss[3:]),
+                                 _count(ds[:2] + ds[3:]))
+        # No more rows than the capacity can be kept.
+        if ds[2] < min(budget, capacity):
+            raise LengthMismatch("compacted cache positions", min(budget, capacity), ds[2])
+        size = src.element_size()
+        width = 1
+        if src.dim() == 4:
+            width = ss[3]
+            if src.numel() and width > 1 and (src.stride(3) != 1 or dst.stride(3) != 1):
+                raise BadArgument("elements of a cache row must be neighbours")
+        r.src, r.dst, r.row_bytes = src.data_ptr(), dst.data_ptr(), width * size
+        st, dt = src.stride(), dst.stride()
+        r.src_stride_b, r.src_stride_h, r.src_stride_s = st[0] * size, st[1] * size, st[2] * size
+        r.dst_stride_b, r.dst_stride_h, r.dst_stride_s = dt[0] * size, dt[1] * size, dt[2] * size
+    call(launch, _lib.lib().rsort_cache_compact, rows, len(sources), kept.data_ptr(),
+         kept_lengths.data_ptr(), batch, heads, budget, capacity)
