@@ -523,7 +523,7 @@ rsort_status rsort_keys_static(rsort_key_t key, int descending, void *d_keys, si
  * rsort_expert_rows(nslots, experts, align) rows hold any outcome (0: the
  * sizes are not supported; at most RSORT_MAX_EXPERTS experts, an align of at
  * most RSORT_MAX_EXPERT_ALIGN and 2^31 - 1 rows).  d_scratch holds
- * rsort_expert_sort_scratch_bytes(nslots, experts) bytes, 4-byte aligned, and
+ * rsort_expert_sort_scratch_bytes(nslots, experts) bytes, 16-byte aligned, and
  * serves one call at a time.
  *
  *   rsort_expert_gather   rows[row_of_slot[t, k]] = x[t] for every kept slot

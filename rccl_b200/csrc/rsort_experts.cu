@@ -17,17 +17,31 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // Counting sort of slots by expert
+//
+// Bound by latency at every size a router produces (512 Ki slots are 8.5 MB).
+// A CTA takes its slots in steps of 32 a warp, SORT_STEPS of them in registers:
+// a warp ranks its slots among its own by votes and keeps a counter per expert,
+// a scan over the warps and one over the experts turn the counters into rows,
+// and every slot adds its rank.  No atomic's order reaches a result.
+//   up to SORT_MAX_CLUSTER CTAs: one launch of one cluster; its CTAs read one
+//     another's counts through distributed shared memory.
+//   longer: a first kernel counts the experts of every CTA's chunk, the second
+//     adds up the chunks before its own; it starts early and ranks meanwhile.
 // ---------------------------------------------------------------------------
-constexpr int SORT_WARPS = 8;
-constexpr int SORT_BLOCK = SORT_WARPS * 32;
+constexpr uint32_t SORT_STEPS = 4;
+constexpr uint32_t SORT_MAX_WARPS = 32;
+constexpr uint32_t SORT_MAX_CLUSTER = 8;
+constexpr uint32_t SORT_MAX_GRID = 1024;  // scratch is sized for this many CTAs
 
 struct SortArgs {
     const void *ids;
     uint32_t n;        // slots
     uint32_t experts;
     uint32_t align;
-    uint32_t chunk;    // slots per CTA, a multiple of SORT_BLOCK
-    uint32_t *counts_of_block;  // [grid][experts]
+    uint32_t id_bits;  // of 0..experts
+    uint32_t chunk;    // slots per CTA, a multiple of SORT_STEPS * its threads
+    uint32_t *counts_of_block;  // [grid][pitch]; null with one cluster
+    uint32_t pitch;    // experts rounded up to 4
     int32_t *row_of_slot, *slot_of_row;
     uint32_t rows;     // capacity of slot_of_row
     int32_t *offsets, *counts;
@@ -35,129 +49,253 @@ struct SortArgs {
 
 // The slot's bucket: its expert, or `experts` for a dropped slot.
 template <typename I>
-__device__ __forceinline__ uint32_t bucket(const SortArgs &a, uint32_t i) {
+__device__ __forceinline__ uint32_t bucket(const SortArgs &a, uint64_t i) {
     const I id = static_cast<const I *>(a.ids)[i];
     return id >= 0 && id < I(a.experts) ? uint32_t(id) : a.experts;
 }
 
-template <typename I>
-__global__ void __launch_bounds__(SORT_BLOCK) expert_count_kernel(const SortArgs a) {
-    extern __shared__ uint32_t hist[];  // experts + 1
-    for (uint32_t e = threadIdx.x; e <= a.experts; e += SORT_BLOCK) hist[e] = 0;
-    __syncthreads();
-    const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
-    const uint64_t last = min(first + a.chunk, uint64_t(a.n));
-    for (uint64_t i = first + threadIdx.x; i < last; i += SORT_BLOCK)
-        atomicAdd(&hist[bucket<I>(a, uint32_t(i))], 1u);
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.experts; e += SORT_BLOCK)
-        a.counts_of_block[size_t(blockIdx.x) * a.experts + e] = hist[e];
+// Every row starts without a slot; the placed ones are overwritten.
+__device__ __forceinline__ void clear_rows(const SortArgs &a) {
+    for (uint64_t r = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; r < a.rows;
+         r += uint64_t(gridDim.x) * blockDim.x)
+        a.slot_of_row[r] = -1;
 }
 
 template <typename I>
-__global__ void __launch_bounds__(SORT_BLOCK) expert_place_kernel(const SortArgs a) {
-    extern __shared__ uint32_t shared[];
-    const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t *const base = shared;                  // [SORT_WARPS][E + 1]
-    uint32_t *const start = base + SORT_WARPS * (E + 1);  // [E + 1] padded offsets
-    uint32_t *const total = start + E + 1;          // [E]
-    __shared__ uint32_t warp_sums[SORT_WARPS];
-    for (uint32_t i = tid; i < SORT_WARPS * (E + 1); i += SORT_BLOCK) base[i] = 0;
+__global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_count_kernel(const SortArgs a) {
+    extern __shared__ uint32_t hist[];  // experts + 1
+    // The placing kernel may start: it waits for this one before it reads.
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (uint32_t e = threadIdx.x; e <= a.experts; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-
-    // Counts of this CTA's warps; each warp owns consecutive slots.
-    const uint64_t first = uint64_t(blockIdx.x) * a.chunk + uint64_t(warp) * (a.chunk / SORT_WARPS);
-    const uint64_t last = min(first + a.chunk / SORT_WARPS, uint64_t(a.n));
-    uint32_t *const mine = base + warp * (E + 1);
-    for (uint64_t i = first + lane; i < last; i += 32)
-        atomicAdd(&mine[bucket<I>(a, uint32_t(i))], 1u);
+    const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
+    const uint64_t last = min(first + a.chunk, uint64_t(a.n));
+#pragma unroll 4
+    for (uint64_t i = first + threadIdx.x; i < last; i += blockDim.x)
+        atomicAdd(&hist[bucket<I>(a, i)], 1u);
+    clear_rows(a);
     __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.pitch; e += blockDim.x)
+        a.counts_of_block[size_t(blockIdx.x) * a.pitch + e] = e < a.experts ? hist[e] : 0;
+}
 
-    // Totals over all CTAs and the part of the earlier ones, then the warps'
-    // running counts inside this CTA.
-    for (uint32_t e = tid; e < E; e += SORT_BLOCK) {
-        uint32_t before = 0, all = 0;
-        for (uint32_t c = 0; c < gridDim.x; ++c) {
-            const uint32_t v = a.counts_of_block[size_t(c) * E + e];
-            if (c < blockIdx.x) before += v;
-            all += v;
-        }
-        total[e] = all;
-        for (uint32_t w = 0; w < SORT_WARPS; ++w) {
-            const uint32_t v = base[w * (E + 1) + e];
-            base[w * (E + 1) + e] = before;
-            before += v;
-        }
+// Lanes of the warp with the same bucket: one vote a bit of the id (on sm_100
+// a vote issues every three cycles and __match_any_sync every sixty).
+__device__ __forceinline__ uint32_t same_bucket(uint32_t e, uint32_t bits) {
+    uint32_t peers = 0xffffffffu;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = (e >> b) & 1u;
+        const uint32_t v = __ballot_sync(0xffffffffu, set);
+        peers &= set ? v : ~v;
     }
-    __syncthreads();
+    return peers;
+}
 
-    // Exclusive scan of the padded segment sizes, SORT_BLOCK experts a step.
-    uint32_t carry = 0;
-    for (uint32_t e0 = 0; e0 < E; e0 += SORT_BLOCK) {
-        const uint32_t e = e0 + tid;
-        const uint32_t size = e < E ? (total[e] + a.align - 1) / a.align * a.align : 0;
-        uint32_t inc = size;
+// Exclusive scan over one value a thread; *total gets the block's sum.
+__device__ __forceinline__ uint32_t sort_scan(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
-            if (lane >= uint32_t(off)) inc += y;
-        }
-        if (lane == 31) warp_sums[warp] = inc;
-        __syncthreads();
-        uint32_t sum = carry;
-        for (uint32_t w = 0; w < SORT_WARPS; ++w) {
-            if (w == warp && e < E) start[e] = sum + inc - size;
-            sum += warp_sums[w];
-        }
-        carry = sum;
-        __syncthreads();
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= uint32_t(off)) inc += y;
     }
-    if (tid == 0) start[E] = carry;
+    if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
+    uint32_t sums = lane < (blockDim.x >> 5) ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, sums, off);
+        if (lane >= uint32_t(off)) sums += y;
+    }
+    *total = __shfl_sync(0xffffffffu, sums, 31);
+    const uint32_t lower = __shfl_sync(0xffffffffu, sums, (warp - 1) & 31);
+    __syncthreads();  // warp_sums may be written again
+    return (warp ? lower : 0) + inc - v;
+}
 
-    // Rows of this warp's slots: lanes with the same expert take consecutive
-    // rows in lane order, so the order of the slots is kept.
-    for (uint64_t i0 = first; i0 < last; i0 += 32) {
-        const uint64_t i = i0 + lane;
-        const bool in = i < last;
-        const uint32_t e = in ? bucket<I>(a, uint32_t(i)) : E;
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        const uint32_t rank = __popc(peers & ((1u << lane) - 1));
-        const uint32_t at = mine[e];
-        __syncwarp();
-        if (rank == 0) mine[e] = at + __popc(peers);
-        __syncwarp();
-        if (in) {
+template <typename I>
+__global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_place_kernel(const SortArgs a) {
+    extern __shared__ uint32_t shared[];
+    __shared__ uint32_t warp_sums[SORT_MAX_WARPS];
+    const uint32_t E = a.experts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t warps = blockDim.x >> 5, pitch = (E + 2) & ~1u;
+    uint32_t *const sub = shared;        // [E] slots of this CTA's current part
+    uint32_t *const total = sub + E;     // [E] slots of the expert
+    uint32_t *const first = total + E;   // [E] first row of this CTA's slots
+    // [warps][pitch] slots of a warp, then of the warps before it
+    uint16_t *const base = reinterpret_cast<uint16_t *>(first + E);
+    uint16_t *const mine = base + warp * pitch;
+    const uint64_t begin = uint64_t(blockIdx.x) * a.chunk;
+    const uint64_t end = min(begin + a.chunk, uint64_t(a.n));
+    const uint32_t part = SORT_STEPS * blockDim.x;  // slots taken at once
+
+    for (uint64_t p = begin; p == begin || p < end; p += part) {
+        const uint64_t slot0 = p + uint64_t(warp) * (SORT_STEPS * 32) + lane;
+        uint32_t e[SORT_STEPS], rank[SORT_STEPS];
+#pragma unroll
+        for (uint32_t k = 0; k < SORT_STEPS; ++k)
+            e[k] = slot0 + 32 * k < end ? bucket<I>(a, slot0 + 32 * k) : E;
+        for (uint32_t i = tid; i < warps * pitch / 2; i += blockDim.x)
+            reinterpret_cast<uint32_t *>(base)[i] = 0;
+        if (p == begin) {
+            for (uint32_t i = tid; i < E; i += blockDim.x) total[i] = first[i] = 0;
+            if (!a.counts_of_block) clear_rows(a);
+        }
+        __syncthreads();
+        // Ranks among the warp's slots: lanes with the same expert in lane
+        // order, step after step.
+#pragma unroll
+        for (uint32_t k = 0; k < SORT_STEPS; ++k) {
+            const uint32_t peers = same_bucket(e[k], a.id_bits);
+            const uint32_t below = __popc(peers & ((1u << lane) - 1));
+            const uint32_t at = mine[e[k]];
+            __syncwarp();
+            if (below == 0) mine[e[k]] = uint16_t(at + __popc(peers));
+            __syncwarp();
+            rank[k] = at + below;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < E; i += blockDim.x) {
+            uint32_t at = 0;
+            for (uint32_t w0 = 0; w0 < warps; w0 += 8) {
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t w = 0; w < 8; ++w)
+                    v[w] = w0 + w < warps ? base[(w0 + w) * pitch + i] : 0;
+#pragma unroll
+                for (uint32_t w = 0; w < 8; ++w) {
+                    if (w0 + w < warps) base[(w0 + w) * pitch + i] = uint16_t(at);
+                    at += v[w];
+                }
+            }
+            sub[i] = at;
+        }
+        if (p == begin) {
+            // The experts' totals and the slots of the CTAs before this one.
+            if (a.counts_of_block) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                const uint32_t quads = a.pitch / 4, wide = (quads + 31) & ~31u;
+                const uint32_t groups = max(blockDim.x / wide, 1u);
+                const uint4 *const counts = reinterpret_cast<const uint4 *>(a.counts_of_block);
+                for (uint32_t i = tid; i < groups * wide; i += blockDim.x) {
+                    const uint32_t q = i % wide;
+                    if (q >= quads) continue;
+                    uint32_t before[4] = {}, all[4] = {};
+#pragma unroll 8
+                    for (uint32_t c = i / wide; c < gridDim.x; c += groups) {
+                        const uint4 v = counts[size_t(c) * quads + q];
+                        const bool b = c < blockIdx.x;
+                        all[0] += v.x, all[1] += v.y, all[2] += v.z, all[3] += v.w;
+                        before[0] += b ? v.x : 0, before[1] += b ? v.y : 0;
+                        before[2] += b ? v.z : 0, before[3] += b ? v.w : 0;
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        if (4 * q + j >= E) break;
+                        atomicAdd(&total[4 * q + j], all[j]);
+                        atomicAdd(&first[4 * q + j], before[j]);
+                    }
+                }
+                __syncthreads();
+            } else {
+                cluster_sync();  // everyone's `sub`, and the cleared rows
+                for (uint32_t i = tid; i < E; i += blockDim.x) {
+                    uint32_t before = 0, all = 0;
+#pragma unroll
+                    for (uint32_t c = 0; c < SORT_MAX_CLUSTER; ++c) {
+                        if (c >= gridDim.x) break;
+                        const uint32_t v = cluster_read(&sub[i], c);
+                        before += c < blockIdx.x ? v : 0;
+                        all += v;
+                    }
+                    total[i] = all;
+                    first[i] = before;
+                }
+                cluster_arrive();  // waited for at the end: `sub` stays until all have read
+                __syncthreads();
+            }
+            // Scan of the padded segment sizes, a block of experts a step.
+            uint32_t carry = 0;
+            for (uint32_t e0 = 0; e0 < E; e0 += blockDim.x) {
+                const uint32_t i = e0 + tid, count = i < E ? total[i] : 0;
+                uint32_t sum;
+                const uint32_t at =
+                    carry + sort_scan((count + a.align - 1) / a.align * a.align, warp_sums, &sum);
+                carry += sum;
+                if (i < E) {
+                    first[i] += at;
+                    if (blockIdx.x == 0) {
+                        a.offsets[i] = int32_t(at);
+                        a.counts[i] = int32_t(count);
+                    }
+                }
+            }
+            if (blockIdx.x == 0 && tid == 0) a.offsets[E] = int32_t(carry);
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < SORT_STEPS; ++k) {
+            const uint64_t i = slot0 + 32 * k;
+            if (i >= end) continue;
             int32_t row = -1;
-            if (e < E) {
-                row = int32_t(start[e] + at + rank);
+            if (e[k] < E) {
+                row = int32_t(first[e[k]] + mine[e[k]] + rank[k]);
                 if (uint32_t(row) < a.rows) a.slot_of_row[row] = int32_t(i);
             }
             a.row_of_slot[i] = row;
         }
-    }
-
-    // Padding rows of the experts, the rows behind the last segment, and the
-    // segments themselves.
-    for (uint32_t e = blockIdx.x; e <= E; e += gridDim.x) {
-        const uint32_t lo = e < E ? start[e] + total[e] : start[E];
-        const uint32_t hi = e < E ? start[e + 1] : a.rows;
-        for (uint32_t r = lo + tid; r < hi && r < a.rows; r += SORT_BLOCK) a.slot_of_row[r] = -1;
-    }
-    if (blockIdx.x == 0) {
-        for (uint32_t e = tid; e <= E; e += SORT_BLOCK) {
-            a.offsets[e] = int32_t(start[e]);
-            if (e < E) a.counts[e] = int32_t(total[e]);
+        if (p + part < end) {
+            __syncthreads();
+            for (uint32_t i = tid; i < E; i += blockDim.x) first[i] += sub[i];
+            __syncthreads();
         }
     }
+    if (!a.counts_of_block) cluster_wait();
 }
 
-uint32_t sort_grid(size_t n, int sm_count) {
-    const size_t want = (n + 1023) / 1024;
-    return uint32_t(want < 1 ? 1 : want < size_t(sm_count) ? want : size_t(sm_count));
+// Warps of a CTA: an eighth of a short input each (ranking and the scattered
+// stores are bound by the SM: 8 Ki slots take 9.3 us on two CTAs of 32 warps,
+// 6.0 us on eight of 8), and at most what leaves the counters 48 KB.
+uint32_t sort_warps(size_t n, size_t experts) {
+    const uint32_t most = experts <= 512 ? 32 : 16;
+    const size_t slots = SORT_MAX_CLUSTER * SORT_STEPS * 32, want = (n + slots - 1) / slots;
+    return uint32_t(want < 4 ? 4 : want < most ? want : most);
 }
 
-constexpr int SORT_MAX_GRID = 1024;  // scratch is sized for this many CTAs
+uint32_t sort_grid(size_t n, size_t experts, uint32_t sms) {
+    const size_t part = size_t(sort_warps(n, experts)) * 32 * SORT_STEPS;
+    const size_t want = (n + part - 1) / part;
+    return uint32_t(want < 1 ? 1 : want < sms ? want : sms);
+}
+
+template <typename I>
+cudaError_t launch_sort(SortArgs a, uint32_t grid, uint32_t warps, cudaStream_t s) {
+    if (a.counts_of_block) {
+        LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
+        expert_count_kernel<I><<<grid, SORT_MAX_WARPS * 32, (a.experts + 1) * 4, s>>>(a);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
+    cudaLaunchAttribute attr{};
+    if (a.counts_of_block) {
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+    } else {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = grid;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = size_t(a.experts) * 12 + size_t(warps) * ((a.experts + 2) & ~1u) * 2;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, expert_place_kernel<I>, a);
+}
 
 // ---------------------------------------------------------------------------
 // Rows in and out of expert order
@@ -385,7 +523,7 @@ size_t rsort_expert_rows(size_t nslots, size_t experts, size_t align) {
 
 size_t rsort_expert_sort_scratch_bytes(size_t nslots, size_t experts) {
     if (experts < 1 || experts > RSORT_MAX_EXPERTS || nslots > size_t(INT_MAX)) return 0;
-    return sort_grid(nslots, SORT_MAX_GRID) * experts * sizeof(uint32_t);
+    return sort_grid(nslots, experts, SORT_MAX_GRID) * ((experts + 3) & ~size_t(3)) * 4;
 }
 
 rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t nslots,
@@ -413,45 +551,38 @@ rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t ns
                                       "expert ids alignment");
     if (st == RSORT_OK)
         st = check_alignment(addr(d_row_of_slot) | addr(d_slot_of_row) | addr(d_offsets) |
-                                 addr(d_counts) | addr(d_scratch),
+                                 addr(d_counts),
                              4, "expert plan alignment");
+    if (st == RSORT_OK) st = check_alignment(addr(d_scratch), 16, "expert sort scratch alignment");
     if (st != RSORT_OK) return st;
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
-    if (sms > SORT_MAX_GRID) sms = SORT_MAX_GRID;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 
+    uint32_t grid =
+        sort_grid(nslots, experts, uint32_t(sms) < SORT_MAX_GRID ? sms : SORT_MAX_GRID);
+    if (grid <= SORT_MAX_CLUSTER)  // clusters of 1, 2, 4 or 8
+        while (grid & (grid - 1)) ++grid;
+    const uint32_t warps = sort_warps(nslots, experts);
+    const size_t part = size_t(warps) * 32 * SORT_STEPS;
     SortArgs a{};
     a.ids = d_ids;
     a.n = uint32_t(nslots);
     a.experts = uint32_t(experts);
     a.align = uint32_t(align);
-    const uint32_t grid = sort_grid(nslots, sms);
-    a.chunk = uint32_t(((nslots + grid - 1) / grid + SORT_BLOCK - 1) / SORT_BLOCK * SORT_BLOCK);
-    a.counts_of_block = static_cast<uint32_t *>(d_scratch);
+    while (experts >> a.id_bits) ++a.id_bits;
+    a.chunk = uint32_t(((nslots + grid - 1) / grid + part - 1) / part * part);
+    a.counts_of_block = grid > SORT_MAX_CLUSTER ? static_cast<uint32_t *>(d_scratch) : nullptr;
+    a.pitch = uint32_t((experts + 3) & ~size_t(3));
     a.row_of_slot = d_row_of_slot;
     a.slot_of_row = d_slot_of_row;
     a.rows = uint32_t(nrows);
     a.offsets = d_offsets;
     a.counts = d_counts;
-    const size_t count_shared = (experts + 1) * 4;
-    const size_t place_shared = (SORT_WARPS * (experts + 1) + 2 * experts + 1) * 4;
-    {
-        LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
-        if (id_type == RSORT_I32)
-            expert_count_kernel<int32_t><<<grid, SORT_BLOCK, count_shared, s>>>(a);
-        else
-            expert_count_kernel<int64_t><<<grid, SORT_BLOCK, count_shared, s>>>(a);
-    }
-    {
-        LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
-        if (id_type == RSORT_I32)
-            expert_place_kernel<int32_t><<<grid, SORT_BLOCK, place_shared, s>>>(a);
-        else
-            expert_place_kernel<int64_t><<<grid, SORT_BLOCK, place_shared, s>>>(a);
-    }
-    return launched(cudaGetLastError(), "expert sort launch");
+    const cudaError_t e = id_type == RSORT_I32 ? launch_sort<int32_t>(a, grid, warps, s)
+                                               : launch_sort<int64_t>(a, grid, warps, s);
+    return launched(e, "expert sort launch");
 }
 
 rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x, size_t x_stride,

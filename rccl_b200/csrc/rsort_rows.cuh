@@ -64,6 +64,31 @@ inline bool rows_fit(size_t n, size_t stride, size_t bytes) {
     return bytes <= kMost && (n == 0 || stride <= kMost / n);
 }
 
+// Thread-block clusters: a word of CTA `rank`'s shared memory at the same
+// place as `p`, and the cluster's barrier in one piece or in two.
+__device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(at)
+        : "r"(uint32_t(__cvta_generic_to_shared(p))), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ uint32_t cluster_read(const uint32_t *p, uint32_t rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_address(p, rank)));
+    return v;
+}
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    cluster_arrive();
+    cluster_wait();
+}
+
 inline rsort_status fail(rsort_status s, const char *role, size_t expected = 0,
                          size_t actual = 0) {
     return record_failure(s, role, expected, actual);

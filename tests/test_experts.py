@@ -72,7 +72,8 @@ def sort_status(**kw):
     (dict(ids=0x1002), _lib.RSORT_BAD_ARGUMENT),
     (dict(t=_lib.RSORT_I64, ids=0x1004), _lib.RSORT_BAD_ARGUMENT),
     (dict(row=0x2001), _lib.RSORT_BAD_ARGUMENT),
-    (dict(scratch=0x6002), _lib.RSORT_BAD_ARGUMENT)])
+    (dict(scratch=0x6002), _lib.RSORT_BAD_ARGUMENT),
+    (dict(scratch=0x6008), _lib.RSORT_BAD_ARGUMENT)])
 def test_sort_refusals(change, status):
     assert sort_status(**change) == status
     assert _lib.last_error().status == status
