@@ -75,15 +75,33 @@ __global__ void __launch_bounds__(ADD_BLOCK) weight_add_kernel(const AddArgs a) 
 
 // ---------------------------------------------------------------------------
 // Selection
+//
+// One cluster of CTAs a head.  Each CTA holds the order images of its slice of
+// the head's totals in registers (totals are read once; only what a slice has
+// beyond SELECT_PAGE is read again), and radix selection finds the
+// smallest kept image in three passes of 11, 11 and 10 bits: a pass counts the
+// digits of the images that still match, and every CTA adds up the cluster's
+// counts through distributed shared memory: 64 sums of 32 bins first, then the
+// one sum's bins (every bin of every CTA took 64 us for 64 heads of 64 Ki
+// positions in clusters of eight, bound by that memory; now 25).  Then a count
+// of the larger and of the equal images of the CTAs and threads before gives
+// every kept position its place, and a page's positions are put in order in shared memory and written
+// out together.  When every image of the found bin stays, the passes below are
+// left out (22 bits tell most totals apart).  Bound by latency: cluster
+// barriers, remote reads and shared-memory atomics of one CTA after another.
 // ---------------------------------------------------------------------------
-constexpr int SELECT_BLOCK = 512;
-constexpr int SELECT_WARPS = SELECT_BLOCK / 32;
+constexpr uint32_t SELECT_BLOCK = 512;
+constexpr uint32_t SELECT_WARPS = SELECT_BLOCK / 32;
+constexpr uint32_t SELECT_BINS = 4 * SELECT_BLOCK;
+constexpr uint32_t SELECT_MAX_CLUSTER = 8;
+constexpr uint32_t SELECT_ITEMS = 16;  // images a thread holds
+constexpr uint32_t SELECT_PAGE = SELECT_ITEMS * SELECT_BLOCK;
 
 struct SelectArgs {
     const float *scores;
     size_t score_b, score_h;
     const int32_t *lengths;
-    uint32_t heads, capacity, budget, sinks, recent;
+    uint32_t heads, capacity, budget, sinks, recent, cluster;
     int32_t *kept, *kept_lengths;
 };
 
@@ -94,90 +112,216 @@ __device__ __forceinline__ uint32_t score_image(float x) {
     return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
-// Exclusive sum over the block of one value a thread; *total gets the sum.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t inc = v;
+// Inclusive sum over the warp.
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {
+    const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= uint32_t(off)) inc += y;
+        const uint32_t y = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= uint32_t(off)) v += y;
     }
-    __syncthreads();  // warp_sums of an earlier scan have been read
-    if (lane == 31) warp_sums[warp] = inc;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < SELECT_WARPS; ++w) {
-        const uint32_t s = warp_sums[w];
-        if (uint32_t(w) < warp) before += s;
-        all += s;
-    }
-    *total = all;
-    return before + inc - v;
+    return v;
 }
 
-// One CTA a head: radix selection of the smallest kept image, eight bits a
-// pass, then one ordered pass that writes the kept positions.
+// Exclusive sum over the block of one value a thread; *total gets the sum.
+__device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t *warp_sums, uint32_t *total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t inc = warp_scan(v);
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    const uint32_t sums = warp_scan(lane < SELECT_WARPS ? warp_sums[lane] : 0);
+    *total = __shfl_sync(0xffffffffu, sums, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, sums, (warp - 1) & 31);
+    return (warp ? before : 0) + inc - v;
+}
+
 __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const SelectArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t warp_sums[SELECT_WARPS];
-    __shared__ uint32_t chosen, left;
-    const uint32_t b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, tid = threadIdx.x;
+    // In turn: a page of images on its way from loads by item to runs of
+    // SELECT_ITEMS a thread, the three passes' counts, a page of positions.
+    __shared__ uint4 shared[(SELECT_PAGE + SELECT_BLOCK) / 4];
+    static_assert(SELECT_PAGE + SELECT_BLOCK >= 3 * SELECT_BINS, "the counts fit");
+    __shared__ uint32_t groups[3][SELECT_BINS / 32], warp_sums[2][SELECT_WARPS];
+    __shared__ uint32_t chosen, left, whole, counts[2];
+    uint32_t *const words = reinterpret_cast<uint32_t *>(shared);
+    const uint32_t row = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;
+    const uint32_t b = row / a.heads, h = row % a.heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t n = length_of(a.lengths, b, a.capacity);
-    int32_t *kept = a.kept + size_t(blockIdx.x) * a.budget;
-    if (h == 0 && tid == 0) a.kept_lengths[b] = int32_t(min(n, a.budget));
+    int32_t *const kept = a.kept + size_t(row) * a.budget;
+    const uint32_t tid_c = rank * SELECT_BLOCK + tid, threads_c = a.cluster * SELECT_BLOCK;
+    if (h == 0 && tid_c == 0) a.kept_lengths[b] = int32_t(min(n, a.budget));
     if (n <= a.budget) {
-        for (uint32_t j = tid; j < a.budget; j += SELECT_BLOCK) kept[j] = j < n ? int32_t(j) : -1;
+        for (uint32_t j = tid_c; j < a.budget; j += threads_c) kept[j] = j < n ? int32_t(j) : -1;
         return;
     }
-    for (uint32_t j = tid; j < a.sinks; j += SELECT_BLOCK) kept[j] = int32_t(j);
-    for (uint32_t j = tid; j < a.recent; j += SELECT_BLOCK)
+    for (uint32_t j = tid_c; j < a.sinks; j += threads_c) kept[j] = int32_t(j);
+    for (uint32_t j = tid_c; j < a.recent; j += threads_c)
         kept[a.budget - a.recent + j] = int32_t(n - a.recent + j);
     const uint32_t need = a.budget - a.sinks - a.recent;
     if (need == 0) return;
-    const float *scores = a.scores + b * a.score_b + h * a.score_h + a.sinks;
-    const uint32_t m = n - a.sinks - a.recent;  // more than need
-    uint32_t prefix = 0, want = need;  // of the images that start with prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = tid; i < 256; i += SELECT_BLOCK) hist[i] = 0;
-        __syncthreads();
-        const uint32_t above = shift == 24 ? 0 : 0xffffffffu << (shift + 8);
-        for (uint32_t i = tid; i < m; i += SELECT_BLOCK) {
-            const uint32_t v = score_image(scores[i]);
-            if ((v & above) == prefix) atomicAdd(&hist[(v >> shift) & 255], 1u);
+
+    // This CTA's slice of the totals between (m is more than need), in pages
+    // of SELECT_ITEMS a thread.  No total has the image 0, so places behind
+    // the slice match nothing below.
+    const float *const scores = a.scores + b * a.score_b + h * a.score_h + a.sinks;
+    const uint32_t m = n - a.sinks - a.recent;
+    const uint32_t per = (m + a.cluster - 1) / a.cluster;
+    const uint32_t lo = min(rank * per, m), len = min(per, m - lo);
+    const uint32_t pages = (len + SELECT_PAGE - 1) / SELECT_PAGE;
+    using Items = uint32_t[SELECT_ITEMS];
+    auto load = [&](uint32_t page, Items &v) {  // item k: position k * SELECT_BLOCK + tid
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k) {
+            const uint32_t i = page * SELECT_PAGE + k * SELECT_BLOCK + tid;
+            v[k] = i < len ? score_image(scores[lo + i]) : 0;
+        }
+    };
+    auto turn = [&](Items &v) {  // item k: position tid * SELECT_ITEMS + k
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k) {
+            const uint32_t i = k * SELECT_BLOCK + tid;
+            words[i + i / SELECT_ITEMS] = v[k];
         }
         __syncthreads();
-        // From the highest digit down: the digit in which the count of kept
-        // images is reached.
-        const uint32_t d = 255 - tid;
-        const uint32_t v = tid < 256 ? hist[d] : 0;
-        uint32_t total;
-        const uint32_t higher = block_scan(v, warp_sums, &total);
-        if (tid < 256 && higher < want && want <= higher + v) {
-            chosen = d;
-            left = want - higher;
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k) v[k] = words[tid * (SELECT_ITEMS + 1) + k];
+        __syncthreads();
+    };
+    Items held;
+    load(0, held);
+    turn(held);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) shared[p * SELECT_BLOCK + tid] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+
+    uint32_t prefix = 0, want = need;  // `want` of the images that start with prefix stay
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const int above = pass == 1 ? 21 : 10;
+        const uint32_t mask = pass == 2 ? 1023 : 2047;
+        uint32_t *const hist = words + pass * SELECT_BINS;
+        auto count = [&](const Items &v) {
+#pragma unroll
+            for (uint32_t k = 0; k < SELECT_ITEMS; ++k)
+                if (pass == 0 ? v[k] != 0 : v[k] >> above == prefix >> above)
+                    atomicAdd(&hist[(v[k] >> shift) & mask], 1u);
+        };
+        count(held);
+        for (uint32_t page = 1; page < pages; ++page) {
+            Items v;
+            load(page, v);
+            count(v);
+        }
+        // This CTA's sums of 32 neighbouring bins: eight threads with four
+        // bins each.
+        __syncthreads();
+        const uint4 q = shared[pass * SELECT_BLOCK + tid];
+        uint32_t sum = q.x + q.y + q.z + q.w;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane % 8 == 0) groups[pass][tid / 8] = sum;
+        if (a.cluster == 1) __syncthreads();
+        else cluster_sync();
+        // One warp adds up the cluster's sums and finds, from the highest
+        // down, the group and then the bin in which the kept count is reached.
+        if (warp == 0) {
+            const uint32_t high =
+                cluster_sum(&groups[pass][63 - 2 * lane], a.cluster);
+            const uint32_t low = cluster_sum(&groups[pass][62 - 2 * lane], a.cluster);
+            uint32_t higher = warp_scan(high + low) - high - low;
+            const bool second = higher + high < want;
+            if (second) higher += high;
+            const uint32_t here = __ballot_sync(
+                0xffffffffu, higher < want && want <= higher + (second ? low : high));
+            const uint32_t from = __ffs(here) - 1;
+            const uint32_t group =
+                __shfl_sync(0xffffffffu, second ? 62 - 2 * lane : 63 - 2 * lane, from);
+            const uint32_t rest = want - __shfl_sync(0xffffffffu, higher, from);
+            const uint32_t bin = group * 32 + 31 - lane;
+            const uint32_t number = cluster_sum(&hist[bin], a.cluster);
+            const uint32_t over = warp_scan(number) - number;
+            if (over < rest && rest <= over + number) {
+                chosen = bin;
+                left = rest - over;
+                whole = rest - over == number;
+            }
         }
         __syncthreads();
         prefix |= chosen << shift;
         want = left;
+        if (whole) {  // every image of the bin stays: the bits below do not matter
+            prefix -= 1;
+            want = 0;
+            break;
+        }
     }
-    // prefix is the smallest kept image; `want` of its equals stay, the lowest
-    // positions first.
-    int32_t *out = kept + a.sinks;
-    uint32_t done = 0, equals = 0;
-    for (uint32_t i0 = 0; i0 < m; i0 += SELECT_BLOCK) {
-        const uint32_t i = i0 + tid;
-        const uint32_t v = i < m ? score_image(scores[i]) : 0;
-        const bool eq = i < m && v == prefix;
-        uint32_t total;
-        const uint32_t rank = equals + block_scan(eq ? 1 : 0, warp_sums, &total);
-        equals += total;
-        const bool keep = i < m && (v > prefix || (eq && rank < want));
-        const uint32_t at = done + block_scan(keep ? 1 : 0, warp_sums, &total);
-        done += total;
-        if (keep && at < need) out[at] = int32_t(a.sinks + i);
+
+    // Images above prefix stay, and `want` of its equals, the lowest positions
+    // first.  Both counts in one word: the larger ones in the low half.
+    auto tally = [&](const Items &v) {
+        uint32_t c = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k)
+            c += (v[k] > prefix ? 1u : 0u) + (v[k] == prefix ? 0x10000u : 0u);
+        return c;
+    };
+    uint32_t total, before = select_scan(tally(held), warp_sums[0], &total);
+    uint32_t larger = total & 0xffff, equal = total >> 16;  // the CTA's
+    for (uint32_t page = 1; page < pages; ++page) {
+        Items v;
+        load(page, v);
+        uint32_t sum;
+        __syncthreads();
+        select_scan(tally(v), warp_sums[1], &sum);
+        larger += sum & 0xffff;
+        equal += sum >> 16;
     }
+    if (a.cluster > 1) {
+        if (tid == 0) {
+            counts[0] = larger;
+            counts[1] = equal;
+        }
+        cluster_sync();
+        larger = equal = 0;
+        for (uint32_t c = 0; c < rank; ++c) {
+            larger += cluster_read(&counts[0], c);
+            equal += cluster_read(&counts[1], c);
+        }
+        cluster_arrive();
+    } else {
+        larger = equal = 0;
+        __syncthreads();  // the last pass's counts have been read
+    }
+    // A page's kept positions are put together and then written in order.
+    auto place = [&](uint32_t page, const Items &v) {
+        const uint32_t first = larger + min(equal, want);
+        uint32_t equals = equal + (before >> 16);
+        uint32_t at = larger + (before & 0xffff) + min(equals, want) - first;
+        const uint32_t i0 = page * SELECT_PAGE + tid * SELECT_ITEMS;
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k) {
+            const bool is_equal = v[k] == prefix;
+            if (v[k] > prefix || (is_equal && equals < want)) words[at++] = a.sinks + lo + i0 + k;
+            equals += is_equal;
+        }
+        larger += total & 0xffff;
+        equal += total >> 16;
+        __syncthreads();
+        const uint32_t number = larger + min(equal, want) - first;
+        int32_t *const out = kept + a.sinks + first;
+        for (uint32_t j = tid; j < number; j += SELECT_BLOCK) out[j] = int32_t(words[j]);
+    };
+    place(0, held);
+    for (uint32_t page = 1; page < pages; ++page) {
+        Items v;
+        load(page, v);
+        __syncthreads();  // the page before has been written
+        turn(v);
+        before = select_scan(tally(v), warp_sums[0], &total);
+        place(page, v);
+    }
+    if (a.cluster > 1) cluster_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -300,6 +444,16 @@ __global__ void __launch_bounds__(MOVE_BLOCK)
         case 2: move_in_place<uint16_t>(r, kept, rows, n, a.capacity, slice); break;
         default: move_in_place<uint8_t>(r, kept, rows, n, a.capacity, slice); break;
     }
+}
+
+// CTAs of a head: enough to hold its totals in registers, as long as all heads
+// run at once (two CTAs an SM).  A CTA costs about 9 us however short its slice:
+// 64 heads of 64 Ki positions take 38 / 25 / 25 us on 2 / 4 / 8 CTAs each (eight
+// need a second wave), 512 heads of 8 Ki 17 / 37 / 76 us on 1 / 2 / 4.
+uint32_t select_cluster(uint32_t rows, uint32_t capacity, uint32_t sms) {
+    uint32_t c = 1;
+    while (c < SELECT_MAX_CLUSTER && capacity / c > SELECT_PAGE && rows * c <= sms) c *= 2;
+    return c;
 }
 
 // batch x heads is a grid dimension of at most 65535.
@@ -459,13 +613,24 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
+    const uint32_t rows = uint32_t(batch * heads);
+    const uint32_t cluster = select_cluster(rows, uint32_t(capacity), uint32_t(sms));
     SelectArgs a{d_scores,           score_stride_b,  score_stride_h,  d_lengths,
                  uint32_t(heads),    uint32_t(capacity), uint32_t(budget), uint32_t(sinks),
-                 uint32_t(recent),   d_kept,          d_kept_lengths};
+                 uint32_t(recent),   cluster,         d_kept,          d_kept_lengths};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
-    cache_select_kernel<<<unsigned(batch * heads), SELECT_BLOCK, 0, s>>>(a);
-    return launched(cudaGetLastError(), "cache selection launch");
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(rows * cluster);
+    cfg.blockDim = dim3(SELECT_BLOCK);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return launched(cudaLaunchKernelEx(&cfg, cache_select_kernel, a), "cache selection launch");
 }
 
 rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,

@@ -78,6 +78,16 @@ __device__ __forceinline__ uint32_t cluster_read(const uint32_t *p, uint32_t ran
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_address(p, rank)));
     return v;
 }
+// The sum of that word over a cluster of at most eight CTAs, read at once.
+__device__ __forceinline__ uint32_t cluster_sum(const uint32_t *p, uint32_t ctas) {
+    if (ctas == 1) return *p;
+    uint32_t v[8], sum = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < 8; ++c) v[c] = c < ctas ? cluster_read(p, c) : 0;
+#pragma unroll
+    for (uint32_t c = 0; c < 8; ++c) sum += v[c];
+    return sum;
+}
 __device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
