@@ -24,8 +24,22 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t b
 
 // ---------------------------------------------------------------------------
 // Totals of attention weights
+//
+// Bound by reading the weights once.  A thread sums V neighbouring positions
+// (16 bytes where the rows allow it) down rows = queries x heads of the group.
+// One query's few rows are summed by one thread; more rows are dealt out to
+// the warps of a CTA and, where the positions alone do not fill the GPU, to the
+// CTAs of a cluster, whose sums meet in (distributed) shared memory in a fixed
+// order.  Two loads a thread in flight (four where rows are dealt out) at four
+// CTAs an SM were best: one query of 64 x 32 heads over 32 Ki positions, bf16,
+// 35 us with 2, 38 with 4, 42 with 8 (201 MB: 5.7 TB/s with 2); 256 queries of
+// 2 x 32 heads over 16 Ki 117 / 110 / 113 us (490 MB: 4.5 TB/s with 4), where
+// 512, 1024 and 2048 bytes of a row side by side take 110, 122 and 150 us.
 // ---------------------------------------------------------------------------
-constexpr int ADD_BLOCK = 256;
+constexpr uint32_t ADD_WARPS = 8;
+constexpr uint32_t ADD_BLOCK = ADD_WARPS * 32;
+constexpr uint32_t ADD_FEW_ROWS = 16;     // summed by one thread
+constexpr uint32_t ADD_MAX_CLUSTER = 8;
 
 struct AddArgs {
     const void *weights;
@@ -33,44 +47,133 @@ struct AddArgs {
     float *scores;
     size_t score_b, score_h;
     const int32_t *lengths;
-    uint32_t heads, group, queries, capacity;
+    uint32_t heads, group, queries, capacity, cluster;
     float decay;
-    int causal;
+    uint32_t causal, score_packs;  // score_packs: rows of totals start on 16 bytes
 };
 
-// One thread sums V neighbouring positions over the group's heads and the
-// queries, in fp32.
-template <typename T, int V>
-__global__ void __launch_bounds__(ADD_BLOCK) weight_add_kernel(const AddArgs a) {
+// Adds rows first, first + step, ... of the group's heads x queries q0.. to acc.
+// ALL: every query sees all V positions.  Else query q sees the positions below
+// end0 + see_more * q.
+template <typename T, int V, uint32_t DEPTH, bool ALL>
+__device__ __forceinline__ void add_rows(const AddArgs &a, const T *w, uint32_t s0, uint32_t q0,
+                                         uint32_t first, uint32_t step, int64_t end0,
+                                         uint32_t see_more, float (&acc)[V]) {
+    const uint32_t seen = a.queries - q0, rows = a.group * seen;
+    const uint32_t step_g = step / seen, step_q = step % seen;
+    uint32_t g = first / seen, q = first % seen;
+    const bool whole = ALL || s0 + V <= a.capacity;  // a full load stays inside the row
+    auto load = [&](Pack<T, V> &v, uint32_t &live) {
+        const T *p = w + g * a.stride_h + size_t(q0 + q) * a.stride_q + s0;
+        if constexpr (!ALL) {
+            const int64_t end = end0 + int64_t(see_more) * (q0 + q);
+            live = end <= s0 ? 0 : uint32_t(min(end - s0, int64_t(V)));
+        }
+        if (whole && (ALL || live)) {
+            v = *reinterpret_cast<const Pack<T, V> *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (uint32_t(i) < live) v.v[i] = p[i];
+        }
+        g += step_g, q += step_q;
+        if (q >= seen) q -= seen, ++g;
+    };
+    auto add = [&](const Pack<T, V> &v, uint32_t live) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            acc[i] += ALL || uint32_t(i) < live ? to_float(v.v[i]) : 0.0f;
+    };
+    uint32_t r = first;
+    for (; r + (DEPTH - 1) * step < rows; r += DEPTH * step) {
+        Pack<T, V> v[DEPTH];
+        uint32_t live[DEPTH];
+#pragma unroll
+        for (uint32_t k = 0; k < DEPTH; ++k) load(v[k], live[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < DEPTH; ++k) add(v[k], live[k]);
+    }
+    Pack<T, V> v[DEPTH - 1];
+    uint32_t live[DEPTH - 1];
+#pragma unroll
+    for (uint32_t k = 0; k < DEPTH - 1; ++k)
+        if (r + k * step < rows) load(v[k], live[k]);
+#pragma unroll
+    for (uint32_t k = 0; k < DEPTH - 1; ++k)
+        if (r + k * step < rows) add(v[k], live[k]);
+}
+
+// SPLIT: the rows are dealt out to the CTA's warps and to the cluster's CTAs;
+// else every thread of the CTA has positions of its own.
+template <typename T, int V, bool SPLIT>
+__global__ void __launch_bounds__(ADD_BLOCK, 4) weight_add_kernel(const AddArgs a) {
     const uint32_t b = blockIdx.y / a.heads, h = blockIdx.y % a.heads;
     const uint32_t n = length_of(a.lengths, b, a.capacity);
-    const uint32_t s0 = (blockIdx.x * ADD_BLOCK + threadIdx.x) * V;
-    if (s0 >= n) return;
+    const uint32_t rank = SPLIT ? blockIdx.x % a.cluster : 0;
+    constexpr uint32_t WIDE = SPLIT ? 32 : ADD_BLOCK;  // threads side by side on a row
+    const uint32_t tile = (SPLIT ? blockIdx.x / a.cluster : blockIdx.x) * (WIDE * V);
+    if (tile >= n) return;  // the whole cluster's tile
+    const uint32_t col = threadIdx.x % WIDE, s0 = tile + col * V;
+    const T *const w = static_cast<const T *>(a.weights) + b * a.stride_b +
+                       size_t(h) * a.group * a.stride_h;
+    // Query q sees the positions below n - queries + 1 + q: the first queries
+    // see nothing of a late tile.
+    const int64_t end0 = a.causal ? int64_t(n) - a.queries + 1 : int64_t(n);
+    uint32_t q0 = 0;
+    if (a.causal && end0 <= int64_t(tile)) q0 = uint32_t(int64_t(tile) - end0 + 1);
     float acc[V] = {};
-    // Query q sees the positions below n - queries + q + 1.
-    const int64_t hidden = a.causal ? int64_t(s0) - (int64_t(n) - a.queries) : 0;
-    const uint32_t q0 = hidden <= 0 ? 0 : uint32_t(hidden);
-    for (uint32_t g = 0; g < a.group; ++g) {
-        const T *w = static_cast<const T *>(a.weights) + b * a.stride_b +
-                     (size_t(h) * a.group + g) * a.stride_h + s0;
-        for (uint32_t q = q0; q < a.queries; ++q) {
-            const uint32_t end = a.causal ? n - a.queries + q + 1 : n;
-            const T *p = w + q * a.stride_q;
-            if (s0 + V <= end) {
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(p);
-#pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += to_float(v.v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (s0 + i < end) acc[i] += to_float(p[i]);
-            }
-        }
+    float *const out = a.scores + b * a.score_b + h * a.score_h;
+    if (q0 < a.queries) {
+        const uint32_t first = SPLIT ? rank * ADD_WARPS + threadIdx.x / WIDE : 0;
+        const uint32_t step = SPLIT ? a.cluster * ADD_WARPS : 1;
+        const uint32_t last = tile + WIDE * V;
+        if (end0 + int64_t(a.causal) * q0 >= int64_t(last))
+            add_rows<T, V, SPLIT ? 4 : 2, true>(a, w, s0, q0, first, step, end0, a.causal, acc);
+        else
+            add_rows<T, V, SPLIT ? 4 : 2, false>(a, w, s0, q0, first, step, end0, a.causal, acc);
     }
-    float *out = a.scores + b * a.score_b + h * a.score_h + s0;
+    if constexpr (!SPLIT) {
+        using P = Pack<float, V < 4 ? V : 4>;
+        if (a.score_packs && s0 + V <= n) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (s0 + i < n) out[i] = fmaf(a.decay, out[i], acc[i]);
+            for (int i = 0; i < V; i += int(sizeof(P) / 4)) {
+                P p = *reinterpret_cast<P *>(out + s0 + i);
+#pragma unroll
+                for (int j = 0; j < int(sizeof(P) / 4); ++j)
+                    p.v[j] = fmaf(a.decay, p.v[j], acc[i + j]);
+                *reinterpret_cast<P *>(out + s0 + i) = p;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (s0 + i < n) out[s0 + i] = fmaf(a.decay, out[s0 + i], acc[i]);
+        }
+    } else {
+        __shared__ float sums[ADD_WARPS][WIDE * V], part[WIDE * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sums[threadIdx.x / WIDE][i * WIDE + col] = acc[i];
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < WIDE * V; c += ADD_BLOCK) {
+            float sum = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < ADD_WARPS; ++k) sum += sums[k][c];
+            part[c] = sum;
+        }
+        if (a.cluster == 1) __syncthreads();
+        else cluster_sync();
+        // Each CTA of the cluster finishes its share of the positions; sum c
+        // is that of position c % WIDE * V + c / WIDE of the tile.
+        for (uint32_t c = threadIdx.x; c < WIDE * V; c += ADD_BLOCK) {
+            const uint32_t s = tile + c % WIDE * V + c / WIDE;
+            if (c / 8 % a.cluster != rank || s >= n) continue;
+            float sum = 0;
+            for (uint32_t k = 0; k < a.cluster; ++k)
+                sum += __uint_as_float(
+                    cluster_read(reinterpret_cast<const uint32_t *>(&part[c]), k));
+            out[s] = fmaf(a.decay, out[s], sum);
+        }
+        if (a.cluster > 1) cluster_sync();  // part stays until all have read it
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -326,8 +429,13 @@ __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const Select
 
 // ---------------------------------------------------------------------------
 // Moving the cache's rows
+//
+// Bound by memory: every moved row is read and written once.  A thread takes
+// MOVE_UNITS accesses of up to 16 bytes, its neighbours the next ones, and all
+// of its reads are in flight before its first write.
 // ---------------------------------------------------------------------------
-constexpr int MOVE_BLOCK = 256;
+constexpr uint32_t MOVE_BLOCK = 256;
+constexpr uint32_t MOVE_UNITS = 8;
 
 struct Rows {
     const char *src;
@@ -340,109 +448,155 @@ struct Rows {
 
 struct MoveArgs {
     Rows rows[RSORT_MAX_CACHES];
-    uint32_t count, batch, heads, budget, capacity;
+    uint32_t count, heads, budget, capacity;
     const int32_t *kept, *kept_lengths;
 };
 
-// A kept position; -1 unless it can be read.
-__device__ __forceinline__ int32_t kept_at(const int32_t *kept, uint32_t j, uint32_t capacity) {
-    const int32_t p = kept[j];
-    return uint32_t(p) < capacity ? p : -1;
-}
+// The accesses of one thread: from the start, every `stride` units of the rows
+// laid end to end.
+struct Walk {
+    uint32_t row, unit, rows_on, units_on, units;
+    __device__ __forceinline__ Walk(uint64_t start, uint32_t stride, uint32_t units) : units(units) {
+        row = uint32_t(start / units);
+        unit = uint32_t(start - uint64_t(row) * units);
+        rows_on = stride / units;
+        units_on = stride % units;
+    }
+    __device__ __forceinline__ void next() {
+        row += rows_on;
+        unit += units_on;
+        if (unit >= units) unit -= units, ++row;
+    }
+};
 
-// Out of place: the accesses of MOVE_BLOCK * MOVE_STEPS row units a CTA.
-constexpr int MOVE_STEPS = 4;
-
+// Out of place: a CTA moves MOVE_BLOCK * MOVE_UNITS accesses; positions that
+// cannot be read do not move.
 template <typename U>
 __device__ __forceinline__ void move_out(const Rows &r, const int32_t *kept, const char *src,
-                                         char *dst, uint32_t n, uint32_t capacity, uint64_t first) {
-    const uint64_t total = uint64_t(n) * r.units;
+                                         char *dst, uint32_t n, uint32_t capacity, uint32_t block) {
+    const Walk start(uint64_t(block) * (MOVE_BLOCK * MOVE_UNITS) + threadIdx.x, MOVE_BLOCK,
+                     r.units);
+    int32_t from[MOVE_UNITS];
+    U v[MOVE_UNITS];
+    Walk at = start;
 #pragma unroll
-    for (int k = 0; k < MOVE_STEPS; ++k) {
-        const uint64_t i = first + uint64_t(k) * MOVE_BLOCK + threadIdx.x;
-        if (i >= total) return;
-        const uint32_t j = uint32_t(i / r.units), u = uint32_t(i - uint64_t(j) * r.units);
-        const int32_t p = kept_at(kept, j, capacity);
-        if (p < 0) continue;
-        reinterpret_cast<U *>(dst + size_t(j) * r.dst_s)[u] =
-            reinterpret_cast<const U *>(src + size_t(p) * r.src_s)[u];
+    for (uint32_t k = 0; k < MOVE_UNITS; ++k) {
+        from[k] = at.row < n ? kept[at.row] : -1;
+        at.next();
+    }
+    at = start;
+#pragma unroll
+    for (uint32_t k = 0; k < MOVE_UNITS; ++k) {
+        if (uint32_t(from[k]) < capacity)
+            v[k] = reinterpret_cast<const U *>(src + size_t(from[k]) * r.src_s)[at.unit];
+        at.next();
+    }
+    at = start;
+#pragma unroll
+    for (uint32_t k = 0; k < MOVE_UNITS; ++k) {
+        if (uint32_t(from[k]) < capacity)
+            reinterpret_cast<U *>(dst + size_t(at.row) * r.dst_s)[at.unit] = v[k];
+        at.next();
     }
 }
 
-__device__ __forceinline__ const Rows &rows_of_block(const MoveArgs &a, uint32_t *block) {
-    uint32_t t = 0;
-    while (t + 1 < a.count && blockIdx.x >= a.rows[t + 1].first_block) ++t;
-    *block = blockIdx.x - a.rows[t].first_block;
-    return a.rows[t];
-}
-
-__global__ void __launch_bounds__(MOVE_BLOCK)
-    cache_move_kernel(const __grid_constant__ MoveArgs a) {
-    uint32_t block;
-    const Rows &r = rows_of_block(a, &block);
-    const uint32_t bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
-    const uint32_t n = min(length_of(a.kept_lengths, b, a.budget), a.capacity);
-    const int32_t *kept = a.kept + size_t(bh) * a.budget;
-    const char *src = r.src + b * r.src_b + h * r.src_h;
-    char *dst = r.dst + b * r.dst_b + h * r.dst_h;
-    const uint64_t first = uint64_t(block) * (MOVE_BLOCK * MOVE_STEPS);
-    switch (r.access) {
-        case 16: move_out<uint4>(r, kept, src, dst, n, a.capacity, first); break;
-        case 8: move_out<uint2>(r, kept, src, dst, n, a.capacity, first); break;
-        case 4: move_out<uint32_t>(r, kept, src, dst, n, a.capacity, first); break;
-        case 2: move_out<uint16_t>(r, kept, src, dst, n, a.capacity, first); break;
-        default: move_out<uint8_t>(r, kept, src, dst, n, a.capacity, first); break;
-    }
-}
-
-// In place: one CTA walks all rows of a slice of the row's accesses in order.
-// kept[j] >= j, so what a step reads was not written by the steps before it;
-// a barrier lets every read of a step come before its writes.
+// In place: one CTA walks a slice of every row in order, MOVE_BLOCK accesses a
+// step.  kept[j] >= j, so a step's reads may run ahead of the writes of any step
+// before it, but every read of a step has to come before its writes.  Reads go
+// asynchronously into a ring of shared memory, MOVE_UNITS steps ahead, where
+// each thread finds its own again; a barrier a step puts the reads first.
+// (Without the ring a step waited for its reads: 256 heads of 4096 rows of 256
+// bytes, keys and values, took 235 us, and 290 us with the steps of eight CTAs
+// joined by a cluster's barrier.)
 template <typename U>
 __device__ __forceinline__ void move_in_place(const Rows &r, const int32_t *kept, char *rows,
-                                              uint32_t n, uint32_t capacity, uint32_t slice) {
+                                              uint32_t n, uint32_t capacity, uint32_t slice,
+                                              uint4 *ring_memory) {
+    U(*const ring)[MOVE_BLOCK] = reinterpret_cast<U(*)[MOVE_BLOCK]>(ring_memory);
     const uint32_t per = (r.units + r.slices - 1) / r.slices;
-    const uint32_t u0 = slice * per, u1 = min(u0 + per, r.units);
-    if (u0 >= u1) return;
-    const uint64_t total = uint64_t(n) * (u1 - u0);
-    for (uint64_t i0 = 0; i0 < total; i0 += MOVE_BLOCK * MOVE_STEPS) {
-        U v[MOVE_STEPS];
-        U *to[MOVE_STEPS];
+    const uint32_t first = slice * per, units = min(per, r.units - min(first, r.units));
+    if (units == 0 || n == 0 || kept[n - 1] == int32_t(n - 1)) return;  // nothing moves
+    // Rows that stay in front: kept[j] == j up to some row, as positions ascend.
+    const uint32_t hop = (n + MOVE_BLOCK - 1) / MOVE_BLOCK, probe = threadIdx.x * hop;
+    const uint32_t same = __syncthreads_count(probe < n && kept[probe] == int32_t(probe));
+    const uint32_t skip = same ? (same - 1) * hop : 0;
+    kept += skip;
+    rows += skip * r.src_s + first * sizeof(U);
+    n -= skip;
+    capacity -= skip;
+
+    const uint32_t slot = uint32_t(__cvta_generic_to_shared(&ring[0][threadIdx.x]));
+    constexpr uint32_t SLOTS = sizeof(U) * MOVE_BLOCK;
+    Walk look(threadIdx.x, MOVE_BLOCK, units), load = look, store = look;
+    int32_t from[MOVE_UNITS], ahead[MOVE_UNITS];
+    auto read_kept = [&](int32_t(&f)[MOVE_UNITS]) {
 #pragma unroll
-        for (int k = 0; k < MOVE_STEPS; ++k) {
-            const uint64_t i = i0 + uint64_t(k) * MOVE_BLOCK + threadIdx.x;
-            to[k] = nullptr;
-            if (i < total) {
-                const uint32_t j = uint32_t(i / (u1 - u0));
-                const uint32_t u = u0 + uint32_t(i - uint64_t(j) * (u1 - u0));
-                const int32_t p = kept_at(kept, j, capacity);
-                if (p > int32_t(j)) {
-                    v[k] = reinterpret_cast<const U *>(rows + size_t(p) * r.src_s)[u];
-                    to[k] = reinterpret_cast<U *>(rows + size_t(j) * r.src_s) + u;
-                }
-            }
+        for (uint32_t k = 0; k < MOVE_UNITS; ++k) {
+            f[k] = look.row < n ? int32_t(uint32_t(kept[look.row]) - skip) : -1;
+            look.next();
         }
-        __syncthreads();
+    };
+    // The read of one access, if it moves; a group of its own either way.
+    auto read = [&](uint32_t k, int32_t at) {
+        if (uint32_t(at) < capacity && at > int32_t(load.row)) {
+            const char *p = rows + size_t(at) * r.src_s + load.unit * sizeof(U);
+            if constexpr (sizeof(U) >= 4)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(slot + k * SLOTS),
+                             "l"(p), "n"(sizeof(U) < 4 ? 4 : sizeof(U))
+                             : "memory");
+            else
+                ring[k][threadIdx.x] = *reinterpret_cast<const U *>(p);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        load.next();
+    };
+    read_kept(from);
 #pragma unroll
-        for (int k = 0; k < MOVE_STEPS; ++k)
-            if (to[k]) *to[k] = v[k];
+    for (uint32_t k = 0; k < MOVE_UNITS; ++k) read(k, from[k]);
+    read_kept(ahead);
+    const uint64_t total = uint64_t(n) * units;
+    for (uint64_t i = 0; i < total; i += MOVE_BLOCK * MOVE_UNITS) {
+        int32_t after[MOVE_UNITS];
+        read_kept(after);
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_UNITS; ++k) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(MOVE_UNITS - 1) : "memory");
+            __syncthreads();
+            if (uint32_t(from[k]) < capacity && from[k] > int32_t(store.row))
+                reinterpret_cast<U *>(rows + size_t(store.row) * r.src_s)[store.unit] =
+                    ring[k][threadIdx.x];
+            store.next();
+            read(k, ahead[k]);
+            from[k] = ahead[k];
+            ahead[k] = after[k];
+        }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(MOVE_BLOCK)
-    cache_move_in_place_kernel(const __grid_constant__ MoveArgs a) {
-    uint32_t slice;
-    const Rows &r = rows_of_block(a, &slice);
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(MOVE_BLOCK) cache_move_kernel(const __grid_constant__ MoveArgs a) {
+    uint32_t t = 0;
+    while (t + 1 < a.count && blockIdx.x >= a.rows[t + 1].first_block) ++t;
+    const Rows &r = a.rows[t];
+    const uint32_t block = blockIdx.x - r.first_block;
     const uint32_t bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
     const uint32_t n = min(length_of(a.kept_lengths, b, a.budget), a.capacity);
-    const int32_t *kept = a.kept + size_t(bh) * a.budget;
-    char *rows = r.dst + b * r.dst_b + h * r.dst_h;
+    const int32_t *const kept = a.kept + size_t(bh) * a.budget;
+    const char *const src = r.src + b * r.src_b + h * r.src_h;
+    char *const dst = r.dst + b * r.dst_b + h * r.dst_h;
+    __shared__ uint4 ring[IN_PLACE ? MOVE_UNITS * MOVE_BLOCK : 1];
+    auto go = [&](auto unit) {
+        using U = decltype(unit);
+        if constexpr (IN_PLACE) move_in_place<U>(r, kept, dst, n, a.capacity, block, ring);
+        else move_out<U>(r, kept, src, dst, n, a.capacity, block);
+    };
     switch (r.access) {
-        case 16: move_in_place<uint4>(r, kept, rows, n, a.capacity, slice); break;
-        case 8: move_in_place<uint2>(r, kept, rows, n, a.capacity, slice); break;
-        case 4: move_in_place<uint32_t>(r, kept, rows, n, a.capacity, slice); break;
-        case 2: move_in_place<uint16_t>(r, kept, rows, n, a.capacity, slice); break;
-        default: move_in_place<uint8_t>(r, kept, rows, n, a.capacity, slice); break;
+        case 16: go(uint4{}); break;
+        case 8: go(uint2{}); break;
+        case 4: go(uint32_t{}); break;
+        case 2: go(uint16_t{}); break;
+        default: go(uint8_t{}); break;
     }
 }
 
@@ -547,7 +701,7 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
     if (!eb) return fail(RSORT_BAD_ARGUMENT, "attention weight type (f32, f16 or bf16)");
     rsort_status st = check_grid(batch, heads, capacity);
     if (st != RSORT_OK) return st;
-    if (group < 1 || group > size_t(INT_MAX) || queries > size_t(INT_MAX))
+    if (group < 1 || group > size_t(INT_MAX) || queries > size_t(INT_MAX) / group)
         return fail(RSORT_BAD_ARGUMENT, "attention weight heads per cache head or queries");
     if (batch == 0 || heads == 0 || capacity == 0) return RSORT_OK;
     if ((queries && !d_weights) || !d_scores) return fail(RSORT_BAD_ARGUMENT, "null buffer");
@@ -571,17 +725,36 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
     AddArgs a{d_weights,         stride_b,       stride_h,        stride_q,
               d_scores,          score_stride_b, score_stride_h,  d_lengths,
               uint32_t(heads),   uint32_t(group), uint32_t(queries), uint32_t(capacity),
-              decay,             causal != 0};
+              1,                 decay,          causal != 0,
+              ((addr(d_scores) | score_stride_b * 4 | score_stride_h * 4) & 15) == 0};
     const size_t access =
         access_bytes(addr(d_weights) | stride_b * eb | stride_h * eb | stride_q * eb, 16);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    // Few rows: one thread sums them.
+    // More: warps, and CTAs while the positions leave SMs without work.
+    const size_t rows = group * queries;
+    const bool split = rows > ADD_FEW_ROWS;
     auto go = [&](auto t, auto v) {
         using T = decltype(t);
         constexpr int V = decltype(v)::value;
-        const size_t per = size_t(ADD_BLOCK) * V;
-        const dim3 grid(unsigned((capacity + per - 1) / per), unsigned(batch * heads));
-        weight_add_kernel<T, V><<<grid, ADD_BLOCK, 0, s>>>(a);
-        return cudaGetLastError();
+        const size_t per = size_t(split ? 32 : ADD_BLOCK) * V;
+        const size_t tiles = (capacity + per - 1) / per;
+        if (split)
+            while (a.cluster < ADD_MAX_CLUSTER && a.cluster * ADD_WARPS * 4 < rows &&
+                   tiles * batch * heads * a.cluster < size_t(sms) * 16)
+                a.cluster *= 2;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = a.cluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(tiles * a.cluster), unsigned(batch * heads));
+        cfg.blockDim = dim3(ADD_BLOCK);
+        cfg.stream = s;
+        cfg.attrs = &attr;
+        cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+        return split ? cudaLaunchKernelEx(&cfg, weight_add_kernel<T, V, true>, a)
+                     : cudaLaunchKernelEx(&cfg, weight_add_kernel<T, V, false>, a);
     };
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
     return launched(with_type(type, access, go), "attention weight add launch");
@@ -683,12 +856,12 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
 
     MoveArgs a{};
     a.count = uint32_t(ncaches);
-    a.batch = uint32_t(batch);
     a.heads = uint32_t(heads);
     a.budget = uint32_t(budget);
     a.capacity = uint32_t(capacity);
     a.kept = d_kept;
     a.kept_lengths = d_kept_lengths;
+    constexpr uint64_t per = MOVE_BLOCK * MOVE_UNITS;
     uint64_t blocks = 0;
     for (size_t i = 0; i < ncaches; ++i) {
         const rsort_cache_rows &c = caches[i];
@@ -706,12 +879,16 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
                                          16));
         r.units = uint32_t(c.row_bytes / r.access);
         r.first_block = uint32_t(blocks);
+        r.slices = 1;
         if (in_place) {
-            // Slices of at least 64 bytes.
-            r.slices = uint32_t((c.row_bytes + 63) / 64);
+            // Slices of at least 64 bytes, until there are 16 CTAs an SM: they cost
+            // a full batch little (32 x 8 heads of 4096 rows: 175 / 162 / 168 us for
+            // 4 / 8 / 16 an SM), and when few heads move they shorten the walk (8
+            // heads among 256: 48 / 27 / 17 us).
+            while (bh * ncaches * r.slices < size_t(sms) * 16 && c.row_bytes / r.slices >= 128)
+                r.slices *= 2;
             blocks += r.slices;
         } else {
-            const uint64_t per = MOVE_BLOCK * MOVE_STEPS;
             blocks += (uint64_t(budget) * r.units + per - 1) / per;
         }
         if (blocks > uint64_t(INT_MAX)) return fail(RSORT_SIZE_OVERFLOW, "cache rows");
@@ -720,9 +897,9 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
     const dim3 grid{unsigned(blocks), unsigned(bh)};
     if (in_place)
-        cache_move_in_place_kernel<<<grid, MOVE_BLOCK, 0, s>>>(a);
+        cache_move_kernel<true><<<grid, MOVE_BLOCK, 0, s>>>(a);
     else
-        cache_move_kernel<<<grid, MOVE_BLOCK, 0, s>>>(a);
+        cache_move_kernel<false><<<grid, MOVE_BLOCK, 0, s>>>(a);
     return launched(cudaGetLastError(), "cache compaction launch");
 }
 
