@@ -5,6 +5,7 @@
 // dropped.  The sort is a stable counting sort: slot s of expert e goes to row
 // offsets[e] + (number of earlier slots of e), with every expert's segment
 // padded to a multiple of `align` rows.  The plan stays on the device.
+#include <algorithm>
 #include <climits>
 
 #include "../../include/rsort_b200.h"
@@ -313,9 +314,14 @@ struct Shape {
     uint32_t lanes, token_blocks, units;
 };
 
-Shape shape_of(size_t tokens, size_t units) {
+Shape shape_of(size_t tokens, size_t units, size_t most_tokens = ROW_BLOCK) {
     Shape s{1, 0, uint32_t(units)};
-    while (s.lanes < ROW_BLOCK && s.lanes < units) s.lanes <<= 1;
+    while (s.lanes < ROW_BLOCK && (s.lanes < units || ROW_BLOCK / s.lanes > most_tokens))
+        s.lanes <<= 1;
+    // Half the threads a token where a last, short step would idle many.
+    while (s.lanes > 32 && (units + s.lanes - 1) / s.lanes * s.lanes - units > units / 16 &&
+           2 * ROW_BLOCK / s.lanes <= most_tokens)
+        s.lanes >>= 1;
     const uint32_t per = ROW_BLOCK / s.lanes;
     s.token_blocks = uint32_t((tokens + per - 1) / per);
     return s;
@@ -378,108 +384,222 @@ __device__ __forceinline__ void store_weight(void *w, int type, uint64_t slot, f
     else static_cast<__nv_bfloat16 *>(w)[slot] = __float2bfloat16_rn(v);
 }
 
-// out[t] = sum over k of weight * rows[row of slot], summed in fp32 in the
-// order of k and rounded once.
-template <typename T, int V>
-__global__ void __launch_bounds__(ROW_BLOCK)
-    expert_combine_kernel(const Plan p, const Shape s, const T *rows, size_t rows_stride,
-                          const Weights w, T *out, size_t out_stride) {
-    const uint32_t t = blockIdx.x * (ROW_BLOCK / s.lanes) + threadIdx.x / s.lanes;
-    if (t >= p.tokens) return;
-    using P = Pack<T, V>;
-    P *dst = reinterpret_cast<P *>(out + size_t(t) * out_stride);
-    for (uint32_t u = threadIdx.x % s.lanes; u < s.units; u += s.lanes) {
-        float acc[V] = {};
-#pragma unroll 4
-        for (uint32_t k = 0; k < p.top_k; ++k) {
-            const uint64_t slot = uint64_t(t) * p.top_k + k;
-            const int32_t r = row_at(p, slot);
-            if (r < 0) continue;
-            const P v = reinterpret_cast<const P *>(rows + size_t(r) * rows_stride)[u];
-            const float f = weight_at(w, slot);
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(f, to_float(v.v[i]), acc[i]);
+// Combine and its gradient are bound by reading the rows.  All of a token's
+// rows (up to MOST_SLOTS at a time) are read by a thread before it uses the
+// first, 16 bytes of each, with no branch between the reads; a CTA stays for
+// many tokens, and the next one's slots (rows and weights) come into shared
+// memory while it works on this one.
+constexpr uint32_t SLOTS_HELD = 1024;  // of a block's tokens
+constexpr int MOST_SLOTS = 8;
+
+// CTAs an SM: what the registers of `slots` reads in flight leave room for.
+// One more spills and one fewer leaves too few bytes in flight.  16 Ki tokens of
+// 8 rows of 4096 bf16 (1.21 GB): combine 204 / 184 / 186 us with 2 / 3 / 4
+// (6.5 TB/s; 237 us with a branch a row, 196 us with four rows at a time); its
+// gradient (2.28 GB) 407 / 405 / 485 us with 2 / 3 / 4 (5.6 TB/s).  4 Ki tokens of
+// 4 rows of 5120: 40 / 39 / 37 / 42 us with 3 / 4 / 5 / 6, 71 / 64 / 63 / 72 us
+// with 2 / 3 / 4 / 5.  Rings of asynchronous copies in shared memory were no
+// faster (194 and 466 us): they pay for the reads twice in shared memory.
+constexpr int combine_ctas(int slots) { return slots <= 2 ? 6 : slots <= 4 ? 5 : 4; }
+constexpr int backward_ctas(int slots) {
+    return slots <= 2 ? 5 : slots <= 4 ? 4 : slots <= 6 ? 3 : 2;
+}
+
+// For the CTA's tokens, block by block: work(t, rows, weights, buffer) with the
+// token's slots [k0, k0 + count), filled up to a multiple of SLOTS (row -1 and
+// weight 0 for what has no row), then, behind a barrier, done(t, buffer).  All
+// threads take part, also for tokens behind the last (t >= tokens).
+template <int SLOTS, typename Work, typename Done>
+__device__ __forceinline__ void each_token(const Plan &p, const Shape &s, const Weights &w,
+                                           uint32_t k0, uint32_t count, uint32_t first,
+                                           uint32_t stride, Work work, Done done) {
+    __shared__ int32_t held_rows[2][SLOTS_HELD];
+    __shared__ float held_weights[2][SLOTS_HELD];
+    const uint32_t per = ROW_BLOCK / s.lanes, group = threadIdx.x / s.lanes;
+    const uint32_t lane = threadIdx.x % s.lanes, filled = (count + SLOTS - 1) / SLOTS * SLOTS;
+    const uint32_t at = group * filled;
+    auto row_of = [&](uint32_t t, uint32_t k) {
+        return t < p.tokens && k < count ? row_at(p, uint64_t(t) * p.top_k + k0 + k) : -1;
+    };
+    auto weight_of = [&](uint32_t t, uint32_t k, int32_t row) {
+        return row >= 0 ? weight_at(w, uint64_t(t) * p.top_k + k0 + k) : 0.0f;
+    };
+    auto hold = [&](uint32_t buffer, uint32_t t, uint32_t from) {
+        for (uint32_t k = from; k < filled; k += s.lanes) {
+            const int32_t row = row_of(t, k);
+            held_rows[buffer][at + k] = row;
+            held_weights[buffer][at + k] = weight_of(t, k, row);
         }
-        P o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(acc[i]);
-        dst[u] = o;
+    };
+    const uint32_t step = stride * per;
+    uint32_t t = first * per + group;
+    hold(0, t, lane);
+    __syncthreads();
+    uint32_t now = 0;
+    for (uint32_t b = first; b < s.token_blocks; b += stride, t += step, now ^= 1) {
+        int32_t row = -1;
+        float weight = 0;
+        const bool ahead = b + stride < s.token_blocks && lane < filled;
+        if (ahead) {
+            row = row_of(t + step, lane);
+            weight = weight_of(t + step, lane, row);
+        }
+        work(t, &held_rows[now][at], &held_weights[now][at], now);
+        if (ahead) {
+            held_rows[now ^ 1][at + lane] = row;
+            held_weights[now ^ 1][at + lane] = weight;
+            hold(now ^ 1, t + step, lane + s.lanes);
+        }
+        __syncthreads();
+        done(t, now);
     }
 }
 
-// grad_rows[row of slot] = weight * grad_out[t], grad_w[slot] = the dot
-// product of grad_out[t] and rows[row of slot] in fp32; DOT_K slots a pass.
-constexpr int DOT_K = 8;
+// The access u of a row.  A slot without a row reads row 0, whose values
+// are dropped (kept_row): no branch parts the reads.
+template <typename P, typename T>
+__device__ __forceinline__ P read_row(const T *rows, size_t stride, int32_t row, uint32_t u) {
+    return reinterpret_cast<const P *>(rows + size_t(max(row, 0)) * stride)[u];
+}
+template <typename P> __device__ __forceinline__ P kept_row(const P &v, int32_t row) {
+    P o = v;
+    if constexpr (sizeof(P) >= 4) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(&o);
+#pragma unroll
+        for (int i = 0; i < int(sizeof(P) / 4); ++i) w[i] = row < 0 ? 0u : w[i];
+    } else if (row < 0) {
+        o = P{};
+    }
+    return o;
+}
 
-template <typename T, int V>
-__global__ void __launch_bounds__(ROW_BLOCK)
-    expert_combine_backward_kernel(const Plan p, const Shape s, const T *grad_out,
-                                   size_t grad_out_stride, const T *rows, size_t rows_stride,
-                                   const Weights w, T *grad_rows, size_t grad_rows_stride,
-                                   void *grad_w) {
+// out[t] = sum over k of weight * rows[row of slot], summed in fp32 in the
+// order of k and rounded once.
+template <typename T, int V, int SLOTS>
+__global__ void __launch_bounds__(ROW_BLOCK, combine_ctas(SLOTS))
+    expert_combine_kernel(const Plan p, const Shape s, const T *rows, size_t rows_stride,
+                          const Weights w, T *out, size_t out_stride) {
     using P = Pack<T, V>;
-    if (blockIdx.x >= s.token_blocks) {
-        zero_padding<P>(p, blockIdx.x - s.token_blocks, reinterpret_cast<char *>(grad_rows),
+    each_token<SLOTS>(p, s, w, 0, p.top_k, blockIdx.x, gridDim.x,
+               [&](uint32_t t, const int32_t *row, const float *weight, uint32_t) {
+        if (t >= p.tokens) return;
+        P *const dst = reinterpret_cast<P *>(out + size_t(t) * out_stride);
+        for (uint32_t u = blockIdx.y * s.lanes + threadIdx.x % s.lanes; u < s.units;
+             u += gridDim.y * s.lanes) {
+            float acc[V] = {};
+            for (uint32_t k0 = 0; k0 < (p.rows ? p.top_k : 0); k0 += SLOTS) {
+                P v[SLOTS];
+#pragma unroll
+                for (int k = 0; k < SLOTS; ++k)
+                    v[k] = read_row<P>(rows, rows_stride, row[k0 + k], u);
+#pragma unroll
+                for (int k = 0; k < SLOTS; ++k) {
+                    const P kept = kept_row(v[k], row[k0 + k]);
+                    const float f = weight[k0 + k];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] = fmaf(f, to_float(kept.v[i]), acc[i]);
+                }
+            }
+            P o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(acc[i]);
+            dst[u] = o;
+        }
+    }, [](uint32_t, uint32_t) {});
+}
+
+// grad_rows[row of slot] = weight * grad_out[t], grad_w[slot] = the dot
+// product of grad_out[t] and rows[row of slot] in fp32: one pass over the rows
+// serves both.  A launch takes `count` (at most SLOTS) slots of every token
+// from k0 on.
+template <typename T, int V, int SLOTS>
+__global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(SLOTS))
+    expert_combine_backward_kernel(const Plan p, const Shape s, uint32_t k0, uint32_t count,
+                                   const T *grad_out, size_t grad_out_stride, const T *rows,
+                                   size_t rows_stride, const Weights w, T *grad_rows,
+                                   size_t grad_rows_stride, void *grad_w, uint32_t token_ctas) {
+    using P = Pack<T, V>;
+    if (blockIdx.x >= token_ctas) {
+        zero_padding<P>(p, blockIdx.x - token_ctas, reinterpret_cast<char *>(grad_rows),
                         grad_rows_stride * sizeof(T), s.units);
         return;
     }
-    __shared__ float sums[ROW_BLOCK / 32][DOT_K];
-    const uint32_t t = blockIdx.x * (ROW_BLOCK / s.lanes) + threadIdx.x / s.lanes;
-    const uint32_t lane0 = threadIdx.x % s.lanes;
-    const bool live = t < p.tokens;
-    const P *g = reinterpret_cast<const P *>(grad_out + size_t(live ? t : 0) * grad_out_stride);
-    for (uint32_t k0 = 0; k0 < p.top_k; k0 += DOT_K) {
-        float dot[DOT_K] = {};
-        const uint32_t nk = min(uint32_t(DOT_K), p.top_k - k0);
-        const uint64_t slot0 = uint64_t(t) * p.top_k + k0;
-        if (live) {
-            for (uint32_t u = lane0; u < s.units; u += s.lanes) {
-                const P gv = g[u];
+    // The warps' sums of a token's dot products; a token of fewer threads than
+    // a warp has its sums without them.
+    __shared__ float sums[2][ROW_BLOCK / 32][SLOTS];
+    const uint32_t lane = threadIdx.x % s.lanes, width = min(s.lanes, 32u);
+    each_token<SLOTS>(p, s, w, k0, count, blockIdx.x, token_ctas,
+               [&](uint32_t t, const int32_t *row, const float *weight, uint32_t buffer) {
+        const bool live = t < p.tokens;
+        const P *const g =
+            reinterpret_cast<const P *>(grad_out + size_t(live ? t : 0) * grad_out_stride);
+        float dot[SLOTS] = {};
+        for (uint32_t u = lane; live && p.rows && u < s.units; u += s.lanes) {
+            const P gv = g[u];
+            P v[SLOTS];
+            if (grad_w) {
 #pragma unroll
-                for (int k = 0; k < DOT_K; ++k) {
-                    const int32_t r = uint32_t(k) < nk ? row_at(p, slot0 + k) : -1;
-                    if (r < 0) continue;
-                    if (grad_w) {
-                        const P v = reinterpret_cast<const P *>(rows + size_t(r) * rows_stride)[u];
+                for (int k = 0; k < SLOTS; ++k) v[k] = read_row<P>(rows, rows_stride, row[k], u);
+            }
+            if (grad_rows) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            dot[k] = fmaf(to_float(gv.v[i]), to_float(v.v[i]), dot[k]);
-                    }
-                    if (grad_rows) {
-                        const float f = weight_at(w, slot0 + k);
-                        P o;
+                for (int k = 0; k < SLOTS; ++k) {
+                    const int32_t r = row[k];
+                    const float f = weight[k];
+                    P o;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(f * to_float(gv.v[i]));
+                    for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(f * to_float(gv.v[i]));
+                    if (r >= 0)
                         reinterpret_cast<P *>(grad_rows + size_t(r) * grad_rows_stride)[u] = o;
-                    }
+                }
+            }
+            if (grad_w) {
+#pragma unroll
+                for (int k = 0; k < SLOTS; ++k) {
+                    const P kept = kept_row(v[k], row[k]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        dot[k] = fmaf(to_float(gv.v[i]), to_float(kept.v[i]), dot[k]);
                 }
             }
         }
-        if (!grad_w) continue;
-        // Sum over the token's threads: lanes of a warp first, then warps.
-        const uint32_t width = min(s.lanes, 32u);
+        if (!grad_w) return;
 #pragma unroll
-        for (int k = 0; k < DOT_K; ++k)
+        for (int k = 0; k < SLOTS; ++k)
             for (uint32_t o = width / 2; o > 0; o >>= 1)
                 dot[k] += __shfl_down_sync(0xffffffffu, dot[k], o, width);
         if (s.lanes <= 32) {
-            if (live && lane0 == 0)
-                for (int k = 0; k < DOT_K; ++k)
-                    if (uint32_t(k) < nk) store_weight(grad_w, w.type, slot0 + k, dot[k]);
-            continue;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0)
+            if (live && lane == 0)
 #pragma unroll
-            for (int k = 0; k < DOT_K; ++k) sums[threadIdx.x >> 5][k] = dot[k];
-        __syncthreads();
-        if (live && lane0 < nk) {
-            float total = 0;
-            const uint32_t w0 = threadIdx.x / s.lanes * (s.lanes / 32);
-            for (uint32_t i = 0; i < s.lanes / 32; ++i) total += sums[w0 + i][lane0];
-            store_weight(grad_w, w.type, slot0 + lane0, total);
+                for (int k = 0; k < SLOTS; ++k)
+                    if (uint32_t(k) < count)
+                        store_weight(grad_w, w.type, uint64_t(t) * p.top_k + k0 + k, dot[k]);
+        } else if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k) sums[buffer][threadIdx.x >> 5][k] = dot[k];
         }
-    }
+    }, [&](uint32_t t, uint32_t buffer) {
+        if (!grad_w || s.lanes <= 32 || t >= p.tokens || lane >= count) return;
+        float total = 0;
+        const uint32_t w0 = threadIdx.x / s.lanes * (s.lanes / 32);
+        for (uint32_t i = 0; i < s.lanes / 32; ++i) total += sums[buffer][w0 + i][lane];
+        store_weight(grad_w, w.type, uint64_t(t) * p.top_k + k0 + lane, total);
+    });
+}
+
+// Calls f with the reads that a thread has in flight: all of a token's slots,
+// up to MOST_SLOTS.
+template <typename F> cudaError_t with_slots(uint32_t slots, F f) {
+    if (slots <= 1) return f(std::integral_constant<int, 1>{});
+    if (slots <= 2) return f(std::integral_constant<int, 2>{});
+    if (slots <= 4) return f(std::integral_constant<int, 4>{});
+    if (slots <= 6) return f(std::integral_constant<int, 6>{});
+    return f(std::integral_constant<int, MOST_SLOTS>{});
+}
+
+uint32_t resident(const Shape &shape, int sms, int ctas) {
+    const uint32_t most = uint32_t(sms) * uint32_t(ctas);
+    return shape.token_blocks < most ? shape.token_blocks : most;
 }
 
 // ---------------------------------------------------------------------------
@@ -500,7 +620,8 @@ rsort_status check_plan(const rsort_expert_plan *p, Plan *out) {
     if (!p) return fail(RSORT_BAD_ARGUMENT, "null expert plan");
     if (p->experts < 1 || p->experts > RSORT_MAX_EXPERTS)
         return fail(RSORT_BAD_ARGUMENT, "expert count", RSORT_MAX_EXPERTS, p->experts);
-    if (p->top_k < 1) return fail(RSORT_BAD_ARGUMENT, "expert plan top_k");
+    if (p->top_k < 1 || p->top_k > RSORT_MAX_EXPERTS)
+        return fail(RSORT_BAD_ARGUMENT, "expert plan top_k", RSORT_MAX_EXPERTS, p->top_k);
     if (p->tokens > size_t(INT_MAX) / p->top_k || p->nrows > size_t(INT_MAX))
         return fail(RSORT_SIZE_OVERFLOW, "expert plan (32-bit slots and rows)");
     if (!p->offsets || !p->counts || (p->tokens && !p->row_of_slot))
@@ -664,12 +785,21 @@ rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t typ
                               [&](auto t, auto v) {
                                   using T = decltype(t);
                                   constexpr int V = decltype(v)::value;
-                                  const Shape shape = shape_of(p.tokens, width / V);
-                                  expert_combine_kernel<T, V>
-                                      <<<shape.token_blocks, ROW_BLOCK, 0, s>>>(
+                                  const Shape shape =
+                                      shape_of(p.tokens, width / V, SLOTS_HELD / ((p.top_k + 7) & ~7u));
+                                  // Few tokens: their units on more CTAs.
+                                  uint32_t side = 1;
+                                  while (side * shape.lanes < shape.units &&
+                                         shape.token_blocks * side < uint32_t(sms))
+                                      ++side;
+                                  return with_slots(p.top_k, [&](auto slots) {
+                                      constexpr int S = decltype(slots)::value;
+                                      const dim3 grid(resident(shape, sms, combine_ctas(S)), side);
+                                      expert_combine_kernel<T, V, S><<<grid, ROW_BLOCK, 0, s>>>(
                                           p, shape, static_cast<const T *>(d_rows), rows_stride, w,
                                           static_cast<T *>(d_out), out_stride);
-                                  return cudaGetLastError();
+                                      return cudaGetLastError();
+                                  });
                               }),
                     "expert combine launch");
 }
@@ -728,24 +858,32 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
     if (d_grad_rows) bits |= addr(d_grad_rows) | grad_rows_stride * eb;
     const size_t access = access_bytes(bits, 16);
     const Weights w{d_weights, int(weight_type)};
-    LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
-    return launched(
-        with_type(type, access,
-                  [&](auto t, auto v) {
-                      using T = decltype(t);
-                      constexpr int V = decltype(v)::value;
-                      const Shape shape = shape_of(p.tokens, width / V);
-                      const uint32_t grid =
-                          shape.token_blocks +
-                          (zero_padding_rows && d_grad_rows ? p.experts * PAD_BLOCKS : 0);
-                      if (grid == 0) return cudaSuccess;
-                      expert_combine_backward_kernel<T, V><<<grid, ROW_BLOCK, 0, s>>>(
-                          p, shape, static_cast<const T *>(d_grad_out), grad_out_stride,
-                          static_cast<const T *>(d_rows), rows_stride, w,
-                          static_cast<T *>(d_grad_rows), grad_rows_stride, d_grad_weights);
-                      return cudaGetLastError();
-                  }),
-        "expert combine gradient launch");
+    const auto go = [&](auto t, auto v) {
+        using T = decltype(t);
+        constexpr int V = decltype(v)::value;
+        cudaError_t e = cudaSuccess;
+        for (uint32_t k0 = 0; k0 < p.top_k && e == cudaSuccess; k0 += MOST_SLOTS) {
+            const uint32_t count = std::min(p.top_k - k0, uint32_t(MOST_SLOTS));
+            const Shape shape = shape_of(p.tokens, width / V, SLOTS_HELD / MOST_SLOTS);
+            const uint32_t pad_blocks =
+                k0 == 0 && zero_padding_rows && d_grad_rows ? p.experts * PAD_BLOCKS : 0;
+            e = with_slots(count, [&](auto slots) {
+                constexpr int S = decltype(slots)::value;
+                const uint32_t token_ctas = resident(shape, sms, backward_ctas(S));
+                if (token_ctas + pad_blocks == 0) return cudaSuccess;
+                LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
+                expert_combine_backward_kernel<T, V, S>
+                    <<<token_ctas + pad_blocks, ROW_BLOCK, 0, s>>>(
+                        p, shape, k0, count, static_cast<const T *>(d_grad_out), grad_out_stride,
+                        static_cast<const T *>(d_rows), rows_stride, w,
+                        static_cast<T *>(d_grad_rows), grad_rows_stride, d_grad_weights,
+                        token_ctas);
+                return cudaGetLastError();
+            });
+        }
+        return e;
+    };
+    return launched(with_type(type, access, go), "expert combine gradient launch");
 }
 
 }  // extern "C"

@@ -15,6 +15,9 @@ back, so a step can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
+import ctypes
+import math
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -28,20 +31,33 @@ from .experts import _on, call, real_code
 def _int32(role: str, t: torch.Tensor, *shape: int) -> None:
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise BadArgument(f"{role} must be contiguous int32")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise LengthMismatch(role, _count(shape), t.numel())
 
 
 def _count(shape) -> int:
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+    return math.prod(shape)
+
+
+_ROWS = struct.Struct("9N")  # rsort_cache_rows
+assert _ROWS.size == ctypes.sizeof(_lib.CacheRows)
+
+
+def _rows(t: torch.Tensor):
+    """Address, shape, row width, element size and strides of a cache."""
+    shape, strides, width = t.shape, t.stride(), 1
+    if len(shape) == 4:
+        width = shape[3]
+        if width > 1 and strides[3] != 1 and t.numel():
+            raise BadArgument("elements of a cache row must be neighbours")
+    elif len(shape) != 3:
+        raise BadArgument("caches must be (batch, heads, capacity[, width])")
+    return t.data_ptr(), shape, width, t.element_size(), strides
 
 
 def _scores(t: torch.Tensor) -> None:
-    if t.dtype != torch.float32 or t.dim() != 3 or (
-            t.numel() and t.shape[2] != 1 and t.stride(2) != 1):
+    if t.dtype != torch.float32 or t.dim() != 3 or not (
+            t.is_contiguous() or t.numel() == 0 or t.shape[2] == 1 or t.stride(2) == 1):
         raise BadArgument("cache scores must be (batch, heads, capacity) float32 with "
                           "neighbouring positions")
 
@@ -63,24 +79,24 @@ def device_attention_weight_add(launch: Launch, weights: torch.Tensor, scores: t
     code = real_code(weights.dtype)
     _scores(scores)
     batch, heads, capacity = scores.shape
-    if weights.dim() != 4 or (
-            weights.numel() and capacity != 1 and weights.stride(3) != 1):
+    shape, strides = weights.shape, weights.stride()
+    if len(shape) != 4 or (strides[3] != 1 and capacity != 1 and weights.numel()):
         raise BadArgument("attention weights must be (batch, query heads[, queries], capacity) "
                           "with neighbouring positions")
-    if weights.shape[0] != batch:
-        raise LengthMismatch("attention weight batch", batch, weights.shape[0])
-    if weights.shape[3] != capacity:
-        raise LengthMismatch("attention weight positions", capacity, weights.shape[3])
-    group = weights.shape[1] // heads if heads else 1
-    if group * heads != weights.shape[1] or group < 1:
-        raise LengthMismatch("attention weight heads", max(group, 1) * heads, weights.shape[1])
+    if shape[0] != batch:
+        raise LengthMismatch("attention weight batch", batch, shape[0])
+    if shape[3] != capacity:
+        raise LengthMismatch("attention weight positions", capacity, shape[3])
+    group = shape[1] // heads if heads else 1
+    if group * heads != shape[1] or group < 1:
+        raise LengthMismatch("attention weight heads", max(group, 1) * heads, shape[1])
     if lengths is not None:
         _int32("cache lengths", lengths, batch)
-    sb, sh, sq, _ = weights.stride()
-    call(launch, _lib.lib().rsort_attention_weight_add, code, weights.data_ptr(), sb, sh, sq,
-         batch, heads, group, weights.shape[2], capacity,
+    score_b, score_h, _ = scores.stride()
+    call(launch, _lib.lib().rsort_attention_weight_add, code, weights.data_ptr(), *strides[:3],
+         batch, heads, group, shape[2], capacity,
          None if lengths is None else lengths.data_ptr(), decay, int(causal), scores.data_ptr(),
-         scores.stride(0), scores.stride(1))
+         score_b, score_h)
 
 
 def device_cache_select(launch: Launch, scores: torch.Tensor, lengths: Optional[torch.Tensor],
@@ -102,9 +118,10 @@ def device_cache_select(launch: Launch, scores: torch.Tensor, lengths: Optional[
         _int32("cache lengths", lengths, batch)
     if sinks < 0 or recent < 0:
         raise BadArgument(f"{sinks} sinks, {recent} recent positions")
-    call(launch, _lib.lib().rsort_cache_select, scores.data_ptr(), scores.stride(0),
-         scores.stride(1), None if lengths is None else lengths.data_ptr(), batch, heads,
-         capacity, budget, sinks, recent, kept.data_ptr(), kept_lengths.data_ptr())
+    score_b, score_h, _ = scores.stride()
+    call(launch, _lib.lib().rsort_cache_select, scores.data_ptr(), score_b, score_h,
+         None if lengths is None else lengths.data_ptr(), batch, heads, capacity, budget, sinks,
+         recent, kept.data_ptr(), kept_lengths.data_ptr())
 
 
 def device_cache_compact(launch: Launch, kept: torch.Tensor, kept_lengths: torch.Tensor,
@@ -123,37 +140,33 @@ def device_cache_compact(launch: Launch, kept: torch.Tensor, kept_lengths: torch
         raise LengthMismatch("compacted caches", len(sources), len(destinations))
     if len(sources) > _lib.MAX_CACHES:
         raise BadArgument(f"{len(sources)} caches (at most {_lib.MAX_CACHES})")
-    _on(launch, kept, kept_lengths, *sources, *destinations)
+    in_place = destinations is sources
+    _on(launch, kept, kept_lengths, *sources, *(() if in_place else destinations))
     if kept.dim() != 3:
         raise BadArgument("kept positions must be (batch, heads, budget)")
     batch, heads, budget = kept.shape
     _int32("kept positions", kept, batch, heads, budget)
     _int32("kept lengths", kept_lengths, batch)
     capacity = sources[0].shape[2] if sources and sources[0].dim() >= 3 else 0
+    fewest = min(budget, capacity)  # no more rows than the capacity can be kept
     rows = (_lib.CacheRows * max(len(sources), 1))()
-    for r, src, dst in zip(rows, sources, destinations):
-        if src.dim() not in (3, 4) or dst.dim() != src.dim():
-            raise BadArgument("caches must be (batch, heads, capacity[, width])")
-        if dst.dtype != src.dtype:
-            raise BadArgument(f"cache of {src.dtype} into {dst.dtype}")
-        ss, ds = src.shape, dst.shape
-        if ss[0] != batch or ss[1] != heads or ss[2] != capacity:
-            raise LengthMismatch("cache", batch * heads * capacity, ss[0] * ss[1] * ss[2])
-        if ds[0] != batch or ds[1] != heads or ds[3:] != ss[3:]:
-            raise LengthMismatch("compacted cache", _count(ss[:2] + ss[3:]),
-                                 _count(ds[:2] + ds[3:]))
-        # No more rows than the capacity can be kept.
-        if ds[2] < min(budget, capacity):
-            raise LengthMismatch("compacted cache positions", min(budget, capacity), ds[2])
-        size = src.element_size()
-        width = 1
-        if src.dim() == 4:
-            width = ss[3]
-            if src.numel() and width > 1 and (src.stride(3) != 1 or dst.stride(3) != 1):
-                raise BadArgument("elements of a cache row must be neighbours")
-        r.src, r.dst, r.row_bytes = src.data_ptr(), dst.data_ptr(), width * size
-        st, dt = src.stride(), dst.stride()
-        r.src_stride_b, r.src_stride_h, r.src_stride_s = st[0] * size, st[1] * size, st[2] * size
-        r.dst_stride_b, r.dst_stride_h, r.dst_stride_s = dt[0] * size, dt[1] * size, dt[2] * size
+    for i, src in enumerate(sources):
+        pointer, shape, width, size, strides = _rows(src)
+        if shape[0] != batch or shape[1] != heads or shape[2] != capacity:
+            raise LengthMismatch("cache", batch * heads * capacity, _count(shape[:3]))
+        dst_pointer, dst_strides = pointer, strides
+        dst = destinations[i]
+        if dst is not src:
+            if dst.dtype != src.dtype:
+                raise BadArgument(f"cache of {src.dtype} into {dst.dtype}")
+            dst_pointer, dst_shape, _, _, dst_strides = _rows(dst)
+            if dst_shape[:2] != shape[:2] or dst_shape[3:] != shape[3:]:
+                raise LengthMismatch("compacted cache", _count(shape[:2] + shape[3:]),
+                                     _count(dst_shape[:2] + dst_shape[3:]))
+            if dst_shape[2] < fewest:
+                raise LengthMismatch("compacted cache positions", fewest, dst_shape[2])
+        _ROWS.pack_into(rows, i * _ROWS.size, pointer, dst_pointer, width * size,
+                        strides[0] * size, strides[1] * size, strides[2] * size,
+                        dst_strides[0] * size, dst_strides[1] * size, dst_strides[2] * size)
     call(launch, _lib.lib().rsort_cache_compact, rows, len(sources), kept.data_ptr(),
          kept_lengths.data_ptr(), batch, heads, budget, capacity)

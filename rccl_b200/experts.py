@@ -92,32 +92,34 @@ def device_expert_plan(launch: Launch, tokens: int, top_k: int, experts: int,
     nbytes = lib.rsort_expert_sort_scratch_bytes(tokens * top_k, experts)
     if nbytes == 0:
         raise BadArgument(f"{experts} experts (1..{_lib.MAX_EXPERTS}), align {align}")
+    # One allocation for all arrays, each on 16 bytes.
+    sizes = (nbytes // 4, tokens * top_k, rows, experts + 1, experts)
+    starts, end = [], 0
+    for n in sizes:
+        starts.append(end)
+        end += (n + 3) // 4 * 4
     with torch.cuda.stream(launch.stream):
-        def new(*shape, fill=-1, dtype=torch.int32):
-            return torch.full(shape, fill, dtype=dtype, device=launch.device)
-
-        return ExpertPlan(tokens, top_k, experts, align, rows, new(tokens, top_k), new(rows),
-                          new(experts + 1, fill=0), new(experts, fill=0),
-                          new(nbytes, fill=0, dtype=torch.uint8))
+        block = torch.full((end,), -1, dtype=torch.int32, device=launch.device)
+    scratch, row_of_slot, *rest = (block[i:i + n] for i, n in zip(starts, sizes))
+    return ExpertPlan(tokens, top_k, experts, align, rows, row_of_slot.view(tokens, top_k), *rest,
+                      scratch.view(torch.uint8))
 
 
 def _on(launch: Launch, *tensors: Optional[torch.Tensor]) -> None:
     """Rows may be strided, so only the device is checked here."""
+    device = launch.device
     for t in tensors:
-        if t is not None and t.device != launch.device:
-            raise ContextMismatch(f"tensor on {t.device}, launch on {launch.device}")
-
-
-def _device(launch: Launch):
-    """The launch's device as the current one (launches go to the current one)."""
-    return torch.cuda.device(launch.device)
+        if t is not None and t.device != device:
+            raise ContextMismatch(f"tensor on {t.device}, launch on {device}")
 
 
 def call(launch: Launch, entry, *args) -> None:
+    """Calls a C entry on the launch's stream, with the launch's device as the
+    current one (kernels launch there)."""
     if torch.cuda.current_device() == launch.device.index:
         status = entry(*args, launch.stream.cuda_stream)
     else:
-        with _device(launch):
+        with torch.cuda.device(launch.device):
             status = entry(*args, launch.stream.cuda_stream)
     if status:
         raise_for(status)
@@ -125,13 +127,19 @@ def call(launch: Launch, entry, *args) -> None:
 
 def _rows(role: str, t: torch.Tensor, count: int, width: int, at_least: bool = False) -> int:
     """Row stride of a (count, width) tensor whose elements of a row are neighbours."""
-    if t.dim() != 2 or (t.numel() and t.shape[1] != 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) == 2 and t.is_contiguous():
+        stride = shape[1]
+    elif len(shape) == 2 and (t.numel() == 0 or shape[1] == 1 or t.stride(1) == 1):
+        stride = t.stride(0)
+    else:
         raise BadArgument(f"{role} must be 2-D with neighbouring elements in a row")
-    if t.shape[0] < count or (t.shape[0] > count and not at_least):
-        raise LengthMismatch(role, count, t.shape[0])
-    if t.shape[1] != width:
-        raise LengthMismatch(role + " width", width, t.shape[1])
-    return t.stride(0)
+    n, w = shape
+    if n < count or (n > count and not at_least):
+        raise LengthMismatch(role, count, n)
+    if w != width:
+        raise LengthMismatch(role + " width", width, w)
+    return stride
 
 
 def _weights(t: torch.Tensor, plan: ExpertPlan, role: str = "expert weights") -> int:
