@@ -392,6 +392,16 @@ __device__ __forceinline__ void store_weight(void *w, int type, uint64_t slot, f
 constexpr uint32_t SLOTS_HELD = 1024;  // of a block's tokens
 constexpr int MOST_SLOTS = 8;
 
+// Accesses of a row that a thread takes at a time: several where few slots or
+// short accesses leave few bytes in flight, as sums of at most eight elements
+// (1023 tokens of 2 rows of 1001 f32, 4 bytes an access: combine 4.6 us, 8.0 with
+// one at a time; its gradient 6.4 and 9.3 us).
+__host__ __device__ constexpr int columns_of(int elements, int slots) {
+    int c = 1;
+    while (2 * c * slots <= MOST_SLOTS && 2 * c * elements <= 8) c *= 2;
+    return c;
+}
+
 // CTAs an SM: what the registers of `slots` reads in flight leave room for.
 // One more spills and one fewer leaves too few bytes in flight.  16 Ki tokens of
 // 8 rows of 4096 bf16 (1.21 GB): combine 204 / 184 / 186 us with 2 / 3 / 4
@@ -400,9 +410,9 @@ constexpr int MOST_SLOTS = 8;
 // 4 rows of 5120: 40 / 39 / 37 / 42 us with 3 / 4 / 5 / 6, 71 / 64 / 63 / 72 us
 // with 2 / 3 / 4 / 5.  Rings of asynchronous copies in shared memory were no
 // faster (194 and 466 us): they pay for the reads twice in shared memory.
-constexpr int combine_ctas(int slots) { return slots <= 2 ? 6 : slots <= 4 ? 5 : 4; }
-constexpr int backward_ctas(int slots) {
-    return slots <= 2 ? 5 : slots <= 4 ? 4 : slots <= 6 ? 3 : 2;
+constexpr int combine_ctas(int slots) { return slots <= 4 ? 5 : 4; }
+constexpr int backward_ctas(int elements, int slots) {
+    return columns_of(elements, slots) > 1 ? 3 : slots <= 4 ? 4 : slots <= 6 ? 3 : 2;
 }
 
 // For the CTA's tokens, block by block: work(t, rows, weights, buffer) with the
@@ -480,30 +490,42 @@ __global__ void __launch_bounds__(ROW_BLOCK, combine_ctas(SLOTS))
     expert_combine_kernel(const Plan p, const Shape s, const T *rows, size_t rows_stride,
                           const Weights w, T *out, size_t out_stride) {
     using P = Pack<T, V>;
+    constexpr int COLUMNS = columns_of(V, SLOTS);
     each_token<SLOTS>(p, s, w, 0, p.top_k, blockIdx.x, gridDim.x,
                [&](uint32_t t, const int32_t *row, const float *weight, uint32_t) {
         if (t >= p.tokens) return;
         P *const dst = reinterpret_cast<P *>(out + size_t(t) * out_stride);
-        for (uint32_t u = blockIdx.y * s.lanes + threadIdx.x % s.lanes; u < s.units;
-             u += gridDim.y * s.lanes) {
-            float acc[V] = {};
+        const uint32_t wide = gridDim.y * s.lanes;
+        for (uint32_t u0 = blockIdx.y * s.lanes + threadIdx.x % s.lanes; u0 < s.units;
+             u0 += wide * COLUMNS) {
+            float acc[COLUMNS][V] = {};
             for (uint32_t k0 = 0; k0 < (p.rows ? p.top_k : 0); k0 += SLOTS) {
-                P v[SLOTS];
+                P v[COLUMNS][SLOTS];
 #pragma unroll
-                for (int k = 0; k < SLOTS; ++k)
-                    v[k] = read_row<P>(rows, rows_stride, row[k0 + k], u);
+                for (int c = 0; c < COLUMNS; ++c)
 #pragma unroll
-                for (int k = 0; k < SLOTS; ++k) {
-                    const P kept = kept_row(v[k], row[k0 + k]);
-                    const float f = weight[k0 + k];
+                    for (int k = 0; k < SLOTS; ++k)
+                        v[c][k] = read_row<P>(rows, rows_stride, row[k0 + k],
+                                              min(u0 + c * wide, s.units - 1));
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] = fmaf(f, to_float(kept.v[i]), acc[i]);
-                }
+                for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+                    for (int k = 0; k < SLOTS; ++k) {
+                        const P kept = kept_row(v[c][k], row[k0 + k]);
+                        const float f = weight[k0 + k];
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            acc[c][i] = fmaf(f, to_float(kept.v[i]), acc[c][i]);
+                    }
             }
-            P o;
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(acc[i]);
-            dst[u] = o;
+            for (int c = 0; c < COLUMNS; ++c) {
+                if (u0 + c * wide >= s.units) break;
+                P o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(acc[c][i]);
+                dst[u0 + c * wide] = o;
+            }
         }
     }, [](uint32_t, uint32_t) {});
 }
@@ -513,7 +535,7 @@ __global__ void __launch_bounds__(ROW_BLOCK, combine_ctas(SLOTS))
 // serves both.  A launch takes `count` (at most SLOTS) slots of every token
 // from k0 on.
 template <typename T, int V, int SLOTS>
-__global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(SLOTS))
+__global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(V, SLOTS))
     expert_combine_backward_kernel(const Plan p, const Shape s, uint32_t k0, uint32_t count,
                                    const T *grad_out, size_t grad_out_stride, const T *rows,
                                    size_t rows_stride, const Weights w, T *grad_rows,
@@ -527,6 +549,7 @@ __global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(SLOTS))
     // The warps' sums of a token's dot products; a token of fewer threads than
     // a warp has its sums without them.
     __shared__ float sums[2][ROW_BLOCK / 32][SLOTS];
+    constexpr int COLUMNS = columns_of(V, SLOTS);
     const uint32_t lane = threadIdx.x % s.lanes, width = min(s.lanes, 32u);
     each_token<SLOTS>(p, s, w, k0, count, blockIdx.x, token_ctas,
                [&](uint32_t t, const int32_t *row, const float *weight, uint32_t buffer) {
@@ -534,32 +557,38 @@ __global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(SLOTS))
         const P *const g =
             reinterpret_cast<const P *>(grad_out + size_t(live ? t : 0) * grad_out_stride);
         float dot[SLOTS] = {};
-        for (uint32_t u = lane; live && p.rows && u < s.units; u += s.lanes) {
-            const P gv = g[u];
-            P v[SLOTS];
+        for (uint32_t u0 = lane; live && p.rows && u0 < s.units; u0 += s.lanes * COLUMNS) {
+            P gv[COLUMNS], v[COLUMNS][SLOTS];
+#pragma unroll
+            for (int c = 0; c < COLUMNS; ++c) gv[c] = g[min(u0 + c * s.lanes, s.units - 1)];
             if (grad_w) {
 #pragma unroll
-                for (int k = 0; k < SLOTS; ++k) v[k] = read_row<P>(rows, rows_stride, row[k], u);
-            }
-            if (grad_rows) {
+                for (int c = 0; c < COLUMNS; ++c)
 #pragma unroll
-                for (int k = 0; k < SLOTS; ++k) {
+                    for (int k = 0; k < SLOTS; ++k)
+                        v[c][k] = read_row<P>(rows, rows_stride, row[k],
+                                              min(u0 + c * s.lanes, s.units - 1));
+            }
+#pragma unroll
+            for (int c = 0; c < COLUMNS; ++c) {
+                const uint32_t u = u0 + c * s.lanes;
+                if (u >= s.units) break;
+#pragma unroll
+                for (int k = 0; grad_rows && k < SLOTS; ++k) {
                     const int32_t r = row[k];
                     const float f = weight[k];
                     P o;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(f * to_float(gv.v[i]));
+                    for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(f * to_float(gv[c].v[i]));
                     if (r >= 0)
                         reinterpret_cast<P *>(grad_rows + size_t(r) * grad_rows_stride)[u] = o;
                 }
-            }
-            if (grad_w) {
 #pragma unroll
-                for (int k = 0; k < SLOTS; ++k) {
-                    const P kept = kept_row(v[k], row[k]);
+                for (int k = 0; grad_w && k < SLOTS; ++k) {
+                    const P kept = kept_row(v[c][k], row[k]);
 #pragma unroll
                     for (int i = 0; i < V; ++i)
-                        dot[k] = fmaf(to_float(gv.v[i]), to_float(kept.v[i]), dot[k]);
+                        dot[k] = fmaf(to_float(gv[c].v[i]), to_float(kept.v[i]), dot[k]);
                 }
             }
         }
@@ -869,7 +898,7 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
                 k0 == 0 && zero_padding_rows && d_grad_rows ? p.experts * PAD_BLOCKS : 0;
             e = with_slots(count, [&](auto slots) {
                 constexpr int S = decltype(slots)::value;
-                const uint32_t token_ctas = resident(shape, sms, backward_ctas(S));
+                const uint32_t token_ctas = resident(shape, sms, backward_ctas(V, S));
                 if (token_ctas + pad_blocks == 0) return cudaSuccess;
                 LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
                 expert_combine_backward_kernel<T, V, S>
