@@ -107,6 +107,7 @@ __device__ __forceinline__ void add_rows(const AddArgs &a, const T *w, uint32_t 
 // else every thread of the CTA has positions of its own.
 template <typename T, int V, bool SPLIT>
 __global__ void __launch_bounds__(ADD_BLOCK, 4) weight_add_kernel(const AddArgs a) {
+    begin_kernel();
     const uint32_t b = blockIdx.y / a.heads, h = blockIdx.y % a.heads;
     const uint32_t n = length_of(a.lengths, b, a.capacity);
     const uint32_t rank = SPLIT ? blockIdx.x % a.cluster : 0;
@@ -239,6 +240,7 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t *warp_sums,
 }
 
 __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const SelectArgs a) {
+    begin_kernel();
     // In turn: a page of images on its way from loads by item to runs of
     // SELECT_ITEMS a thread, the three passes' counts, a page of positions.
     __shared__ uint4 shared[(SELECT_PAGE + SELECT_BLOCK) / 4];
@@ -576,6 +578,7 @@ __device__ __forceinline__ void move_in_place(const Rows &r, const int32_t *kept
 
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(MOVE_BLOCK) cache_move_kernel(const __grid_constant__ MoveArgs a) {
+    begin_kernel();
     uint32_t t = 0;
     while (t + 1 < a.count && blockIdx.x >= a.rows[t + 1].first_block) ++t;
     const Rows &r = a.rows[t];
@@ -743,18 +746,9 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
             while (a.cluster < ADD_MAX_CLUSTER && a.cluster * ADD_WARPS * 4 < rows &&
                    tiles * batch * heads * a.cluster < size_t(sms) * 16)
                 a.cluster *= 2;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = a.cluster;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(unsigned(tiles * a.cluster), unsigned(batch * heads));
-        cfg.blockDim = dim3(ADD_BLOCK);
-        cfg.stream = s;
-        cfg.attrs = &attr;
-        cfg.numAttrs = a.cluster > 1 ? 1 : 0;
-        return split ? cudaLaunchKernelEx(&cfg, weight_add_kernel<T, V, true>, a)
-                     : cudaLaunchKernelEx(&cfg, weight_add_kernel<T, V, false>, a);
+        const dim3 grid(unsigned(tiles * a.cluster), unsigned(batch * heads));
+        return launch_early(split ? weight_add_kernel<T, V, true> : weight_add_kernel<T, V, false>,
+                            grid, ADD_BLOCK, 0, a.cluster, s, a);
     };
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
     return launched(with_type(type, access, go), "attention weight add launch");
@@ -793,17 +787,9 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
                  uint32_t(recent),   cluster,         d_kept,          d_kept_lengths};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(rows * cluster);
-    cfg.blockDim = dim3(SELECT_BLOCK);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return launched(cudaLaunchKernelEx(&cfg, cache_select_kernel, a), "cache selection launch");
+    return launched(launch_early(cache_select_kernel, dim3(rows * cluster), SELECT_BLOCK, 0, cluster,
+                                 s, a),
+                    "cache selection launch");
 }
 
 rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
@@ -896,10 +882,12 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
     const dim3 grid{unsigned(blocks), unsigned(bh)};
-    if (in_place)
-        cache_move_kernel<true><<<grid, MOVE_BLOCK, 0, s>>>(a);
-    else
-        cache_move_kernel<false><<<grid, MOVE_BLOCK, 0, s>>>(a);
+    if (!in_place)
+        return launched(launch_early(cache_move_kernel<false>, grid, MOVE_BLOCK, 0, 1, s, a),
+                        "cache compaction launch");
+    // Not early: the CTAs of the few heads that move would crowd on the SMs that
+    // happen to be free (8 of 256 heads: 23 us against 16).
+    cache_move_kernel<true><<<grid, MOVE_BLOCK, 0, s>>>(a);
     return launched(cudaGetLastError(), "cache compaction launch");
 }
 

@@ -65,8 +65,7 @@ __device__ __forceinline__ void clear_rows(const SortArgs &a) {
 template <typename I>
 __global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_count_kernel(const SortArgs a) {
     extern __shared__ uint32_t hist[];  // experts + 1
-    // The placing kernel may start: it waits for this one before it reads.
-    asm volatile("griddepcontrol.launch_dependents;");
+    begin_kernel();  // the placing kernel may start: the ids are there
     for (uint32_t e = threadIdx.x; e <= a.experts; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
@@ -131,6 +130,9 @@ __global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_place_kernel(const
     const uint64_t end = min(begin + a.chunk, uint64_t(a.n));
     const uint32_t part = SORT_STEPS * blockDim.x;  // slots taken at once
 
+    // With a counting kernel before it, this one ranks its slots meanwhile:
+    // that kernel waited for what came before.
+    if (!a.counts_of_block) begin_kernel();
     for (uint64_t p = begin; p == begin || p < end; p += part) {
         const uint64_t slot0 = p + uint64_t(warp) * (SORT_STEPS * 32) + lane;
         uint32_t e[SORT_STEPS], rank[SORT_STEPS];
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_place_kernel(const
         if (p == begin) {
             // The experts' totals and the slots of the CTAs before this one.
             if (a.counts_of_block) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");
+                begin_kernel();
                 const uint32_t quads = a.pitch / 4, wide = (quads + 31) & ~31u;
                 const uint32_t groups = max(blockDim.x / wide, 1u);
                 const uint4 *const counts = reinterpret_cast<const uint4 *>(a.counts_of_block);
@@ -274,28 +276,14 @@ template <typename I>
 cudaError_t launch_sort(SortArgs a, uint32_t grid, uint32_t warps, cudaStream_t s) {
     if (a.counts_of_block) {
         LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
-        expert_count_kernel<I><<<grid, SORT_MAX_WARPS * 32, (a.experts + 1) * 4, s>>>(a);
-        const cudaError_t e = cudaGetLastError();
+        const cudaError_t e = launch_early(expert_count_kernel<I>, dim3(grid), SORT_MAX_WARPS * 32,
+                                           (a.experts + 1) * 4, 1, s, a);
         if (e != cudaSuccess) return e;
     }
     LaunchScope scope(RSORT_KERNEL_EXPERT_SORT, s);
-    cudaLaunchAttribute attr{};
-    if (a.counts_of_block) {
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-    } else {
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = grid;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = size_t(a.experts) * 12 + size_t(warps) * ((a.experts + 2) & ~1u) * 2;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, expert_place_kernel<I>, a);
+    return launch_early(expert_place_kernel<I>, dim3(grid), warps * 32,
+                        size_t(a.experts) * 12 + size_t(warps) * ((a.experts + 2) & ~1u) * 2,
+                        a.counts_of_block ? 1 : grid, s, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -350,6 +338,7 @@ template <typename U>
 __global__ void __launch_bounds__(ROW_BLOCK)
     expert_gather_kernel(const Plan p, const Shape s, const char *x, size_t x_stride, char *rows,
                          size_t rows_stride) {
+    begin_kernel();
     if (blockIdx.x >= s.token_blocks) {
         zero_padding<U>(p, blockIdx.x - s.token_blocks, rows, rows_stride, s.units);
         return;
@@ -491,6 +480,7 @@ __global__ void __launch_bounds__(ROW_BLOCK, combine_ctas(SLOTS))
                           const Weights w, T *out, size_t out_stride) {
     using P = Pack<T, V>;
     constexpr int COLUMNS = columns_of(V, SLOTS);
+    begin_kernel();
     each_token<SLOTS>(p, s, w, 0, p.top_k, blockIdx.x, gridDim.x,
                [&](uint32_t t, const int32_t *row, const float *weight, uint32_t) {
         if (t >= p.tokens) return;
@@ -541,6 +531,7 @@ __global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(V, SLOTS))
                                    size_t rows_stride, const Weights w, T *grad_rows,
                                    size_t grad_rows_stride, void *grad_w, uint32_t token_ctas) {
     using P = Pack<T, V>;
+    begin_kernel();
     if (blockIdx.x >= token_ctas) {
         zero_padding<P>(p, blockIdx.x - token_ctas, reinterpret_cast<char *>(grad_rows),
                         grad_rows_stride * sizeof(T), s.units);
@@ -761,10 +752,9 @@ rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x,
     const uint32_t grid = shape.token_blocks + (zero_padding_rows ? p.experts * PAD_BLOCKS : 0);
     if (grid == 0) return RSORT_OK;
     auto go = [&](auto unit) {
-        expert_gather_kernel<decltype(unit)><<<grid, ROW_BLOCK, 0, s>>>(
-            p, shape, static_cast<const char *>(d_x), x_stride, static_cast<char *>(d_rows),
-            rows_stride);
-        return cudaGetLastError();
+        return launch_early(expert_gather_kernel<decltype(unit)>, dim3(grid), ROW_BLOCK, 0, 1, s,
+                            p, shape, static_cast<const char *>(d_x), x_stride,
+                            static_cast<char *>(d_rows), rows_stride);
     };
     LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
     return launched(access == 16  ? go(uint4{})
@@ -824,10 +814,10 @@ rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t typ
                                   return with_slots(p.top_k, [&](auto slots) {
                                       constexpr int S = decltype(slots)::value;
                                       const dim3 grid(resident(shape, sms, combine_ctas(S)), side);
-                                      expert_combine_kernel<T, V, S><<<grid, ROW_BLOCK, 0, s>>>(
+                                      return launch_early(
+                                          expert_combine_kernel<T, V, S>, grid, ROW_BLOCK, 0, 1, s,
                                           p, shape, static_cast<const T *>(d_rows), rows_stride, w,
                                           static_cast<T *>(d_out), out_stride);
-                                      return cudaGetLastError();
                                   });
                               }),
                     "expert combine launch");
@@ -901,13 +891,11 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
                 const uint32_t token_ctas = resident(shape, sms, backward_ctas(V, S));
                 if (token_ctas + pad_blocks == 0) return cudaSuccess;
                 LaunchScope scope(RSORT_KERNEL_EXPERT_ROWS, s);
-                expert_combine_backward_kernel<T, V, S>
-                    <<<token_ctas + pad_blocks, ROW_BLOCK, 0, s>>>(
-                        p, shape, k0, count, static_cast<const T *>(d_grad_out), grad_out_stride,
-                        static_cast<const T *>(d_rows), rows_stride, w,
-                        static_cast<T *>(d_grad_rows), grad_rows_stride, d_grad_weights,
-                        token_ctas);
-                return cudaGetLastError();
+                return launch_early(
+                    expert_combine_backward_kernel<T, V, S>, dim3(token_ctas + pad_blocks),
+                    ROW_BLOCK, 0, 1, s, p, shape, k0, count, static_cast<const T *>(d_grad_out),
+                    grad_out_stride, static_cast<const T *>(d_rows), rows_stride, w,
+                    static_cast<T *>(d_grad_rows), grad_rows_stride, d_grad_weights, token_ctas);
             });
         }
         return e;

@@ -99,6 +99,35 @@ __device__ __forceinline__ void cluster_sync() {
     cluster_wait();
 }
 
+// Programmatic dependent launch: a kernel of these operators may be brought
+// onto the SMs while the one before it on the stream runs out.  Every CTA calls
+// begin_kernel before it touches memory that another kernel may write: it waits
+// until the kernels before are complete, and lets the next one come.
+__device__ __forceinline__ void begin_kernel() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launches a kernel that calls begin_kernel, in clusters of `cluster` CTAs.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, unsigned block, size_t shared,
+                         unsigned cluster, cudaStream_t stream, Args &&...args) {
+    cudaLaunchAttribute attrs[2] = {};
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 inline rsort_status fail(rsort_status s, const char *role, size_t expected = 0,
                          size_t actual = 0) {
     return record_failure(s, role, expected, actual);
