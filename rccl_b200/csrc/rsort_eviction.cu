@@ -31,10 +31,12 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t b
 // the warps of a CTA and, where the positions alone do not fill the GPU, to the
 // CTAs of a cluster, whose sums meet in (distributed) shared memory in a fixed
 // order.  Two loads a thread in flight (four where rows are dealt out) at four
-// CTAs an SM were best: one query of 64 x 32 heads over 32 Ki positions, bf16,
-// 35 us with 2, 38 with 4, 42 with 8 (201 MB: 5.7 TB/s with 2); 256 queries of
-// 2 x 32 heads over 16 Ki 117 / 110 / 113 us (490 MB: 4.5 TB/s with 4), where
-// 512, 1024 and 2048 bytes of a row side by side take 110, 122 and 150 us.
+// CTAs an SM were best: one query of 64 x 32 heads over 32 Ki positions, bf16
+// (201 MB), 33 us with 2 (6.0 TB/s), 38 with 4, 42 with 8; 256 queries of 2 x 32
+// heads over 16 Ki, causal (490 MB), 80 us (6.1 TB/s) with four CTAs an SM's worth
+// of work dealt out, 88 and 94 us with 8 and 16.  Tiles that some queries see only
+// in part are masked behind the reads: with a branch before each read their
+// CTAs ran twice as long as the others (110 us).
 // ---------------------------------------------------------------------------
 constexpr uint32_t ADD_WARPS = 8;
 constexpr uint32_t ADD_BLOCK = ADD_WARPS * 32;
@@ -53,36 +55,40 @@ struct AddArgs {
 };
 
 // Adds rows first, first + step, ... of the group's heads x queries q0.. to acc.
-// ALL: every query sees all V positions.  Else query q sees the positions below
-// end0 + see_more * q.
-template <typename T, int V, uint32_t DEPTH, bool ALL>
+// SEEN_ALL: every query sees all V positions.  Else query q sees the positions
+// below end0 + see_more * q; SEEN_PART: all V lie inside the row and are read,
+// without a branch between the reads; SEEN_EDGE: the row may end among them.
+enum Seen { SEEN_ALL, SEEN_PART, SEEN_EDGE };
+template <typename T, int V, uint32_t DEPTH, Seen SEEN>
 __device__ __forceinline__ void add_rows(const AddArgs &a, const T *w, uint32_t s0, uint32_t q0,
-                                         uint32_t first, uint32_t step, int64_t end0,
-                                         uint32_t see_more, float (&acc)[V]) {
+                                         uint32_t first, uint32_t step, int32_t end0,
+                                         int32_t see_more, float (&acc)[V]) {
     const uint32_t seen = a.queries - q0, rows = a.group * seen;
     const uint32_t step_g = step / seen, step_q = step % seen;
-    uint32_t g = first / seen, q = first % seen;
-    const bool whole = ALL || s0 + V <= a.capacity;  // a full load stays inside the row
+    uint32_t q = first % seen;
+    const T *p = w + first / seen * a.stride_h + size_t(q0 + q) * a.stride_q + s0;
+    const size_t on = step_g * a.stride_h + step_q * a.stride_q;
+    const size_t wrap = a.stride_h - seen * a.stride_q;  // to the next head's first query
     auto load = [&](Pack<T, V> &v, uint32_t &live) {
-        const T *p = w + g * a.stride_h + size_t(q0 + q) * a.stride_q + s0;
-        if constexpr (!ALL) {
-            const int64_t end = end0 + int64_t(see_more) * (q0 + q);
-            live = end <= s0 ? 0 : uint32_t(min(end - s0, int64_t(V)));
+        if constexpr (SEEN != SEEN_ALL) {
+            const int32_t end = end0 + see_more * int32_t(q0 + q);
+            live = end <= int32_t(s0) ? 0 : min(uint32_t(end) - s0, uint32_t(V));
         }
-        if (whole && (ALL || live)) {
+        if constexpr (SEEN != SEEN_EDGE) {
             v = *reinterpret_cast<const Pack<T, V> *>(p);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (uint32_t(i) < live) v.v[i] = p[i];
         }
-        g += step_g, q += step_q;
-        if (q >= seen) q -= seen, ++g;
+        p += on;
+        q += step_q;
+        if (q >= seen) q -= seen, p += wrap;
     };
     auto add = [&](const Pack<T, V> &v, uint32_t live) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            acc[i] += ALL || uint32_t(i) < live ? to_float(v.v[i]) : 0.0f;
+            acc[i] += SEEN == SEEN_ALL || uint32_t(i) < live ? to_float(v.v[i]) : 0.0f;
     };
     uint32_t r = first;
     for (; r + (DEPTH - 1) * step < rows; r += DEPTH * step) {
@@ -128,10 +134,16 @@ __global__ void __launch_bounds__(ADD_BLOCK, 4) weight_add_kernel(const AddArgs 
         const uint32_t first = SPLIT ? rank * ADD_WARPS + threadIdx.x / WIDE : 0;
         const uint32_t step = SPLIT ? a.cluster * ADD_WARPS : 1;
         const uint32_t last = tile + WIDE * V;
+        const auto add = [&](auto seen) {
+            add_rows<T, V, SPLIT ? 4 : 2, decltype(seen)::value>(
+                a, w, s0, q0, first, step, int32_t(end0), int32_t(a.causal), acc);
+        };
         if (end0 + int64_t(a.causal) * q0 >= int64_t(last))
-            add_rows<T, V, SPLIT ? 4 : 2, true>(a, w, s0, q0, first, step, end0, a.causal, acc);
-        else
-            add_rows<T, V, SPLIT ? 4 : 2, false>(a, w, s0, q0, first, step, end0, a.causal, acc);
+            add(std::integral_constant<Seen, SEEN_ALL>{});
+        else if (s0 + V <= a.capacity)
+            add(std::integral_constant<Seen, SEEN_PART>{});
+        else if (s0 < a.capacity)
+            add(std::integral_constant<Seen, SEEN_EDGE>{});
     }
     if constexpr (!SPLIT) {
         using P = Pack<float, V < 4 ? V : 4>;
@@ -744,7 +756,7 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
         const size_t tiles = (capacity + per - 1) / per;
         if (split)
             while (a.cluster < ADD_MAX_CLUSTER && a.cluster * ADD_WARPS * 4 < rows &&
-                   tiles * batch * heads * a.cluster < size_t(sms) * 16)
+                   tiles * batch * heads * a.cluster < size_t(sms) * 4)
                 a.cluster *= 2;
         const dim3 grid(unsigned(tiles * a.cluster), unsigned(batch * heads));
         return launch_early(split ? weight_add_kernel<T, V, true> : weight_add_kernel<T, V, false>,
