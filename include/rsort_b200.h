@@ -521,8 +521,8 @@ rsort_status rsort_keys_static(rsort_key_t key, int descending, void *d_keys, si
  *   slot_of_row[r]  the row's slot, -1 in padding and behind the last segment
  * The plan stays on the device: nothing synchronizes, so it can be captured.
  * rsort_expert_rows(nslots, experts, align) rows hold any outcome (0: the
- * sizes are not supported; at most RSORT_MAX_EXPERTS experts, an align of at
- * most RSORT_MAX_EXPERT_ALIGN and 2^31 - 1 rows).  d_scratch holds
+ * sizes are not supported; at most RSORT_MAX_EXPERTS experts, as many choices of
+ * a token, an align of at most RSORT_MAX_EXPERT_ALIGN and 2^31 - 1 rows).  d_scratch holds
  * rsort_expert_sort_scratch_bytes(nslots, experts) bytes, 16-byte aligned, and
  * serves one call at a time.
  *

@@ -787,8 +787,19 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
     st = check_alignment(addr(d_scores) | addr(d_lengths) | addr(d_kept) | addr(d_kept_lengths), 4,
                          "cache selection alignment");
     if (st != RSORT_OK) return st;
-    if (overlap(rows_range(d_kept_lengths, batch, 4, 4), rows_range(d_lengths, batch, 4, 4)))
+    if (d_lengths &&
+        overlap(rows_range(d_kept_lengths, batch, 4, 4), rows_range(d_lengths, batch, 4, 4)))
         return fail(RSORT_BAD_ARGUMENT, "kept lengths overlap the lengths");
+    Strided scores{};
+    if (!strided(d_scores, batch, heads, capacity, score_stride_b * 4, score_stride_h * 4, 4, 4,
+                 &scores))
+        return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
+    const ByteRange kept = rows_range(d_kept, batch * heads * budget, 4, 4);
+    const ByteRange kept_n = rows_range(d_kept_lengths, batch, 4, 4);
+    const ByteRange read = capacity ? scores.range : ByteRange{0, 0};
+    if (overlap(kept, read) || overlap(kept_n, read) || overlap(kept, kept_n) ||
+        (d_lengths && overlap(kept, rows_range(d_lengths, batch, 4, 4))))
+        return fail(RSORT_BAD_ARGUMENT, "kept positions overlap another buffer");
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;

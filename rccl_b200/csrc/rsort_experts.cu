@@ -584,6 +584,9 @@ __global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(V, SLOTS))
             }
         }
         if (!grad_w) return;
+        // A dropped slot has 0, also where grad_out is not finite.
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) dot[k] = row[k] < 0 ? 0.0f : dot[k];
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k)
             for (uint32_t o = width / 2; o > 0; o >>= 1)
@@ -696,6 +699,19 @@ rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t ns
                              4, "expert plan alignment");
     if (st == RSORT_OK) st = check_alignment(addr(d_scratch), 16, "expert sort scratch alignment");
     if (st != RSORT_OK) return st;
+    const size_t id_bytes = id_type == RSORT_I64 ? 8 : 4;
+    const ByteRange ids = rows_range(d_ids, nslots, id_bytes, id_bytes);
+    const ByteRange written[] = {rows_range(d_row_of_slot, nslots, 4, 4),
+                                 rows_range(d_slot_of_row, nrows, 4, 4),
+                                 rows_range(d_offsets, experts + 1, 4, 4),
+                                 rows_range(d_counts, experts, 4, 4),
+                                 rows_range(d_scratch, bytes, 1, 1)};
+    for (const ByteRange &w : written) {
+        if (overlap(ids, w)) return fail(RSORT_BAD_ARGUMENT, "expert plan overlaps the ids");
+        for (const ByteRange &v : written)
+            if (&v != &w && overlap(v, w))
+                return fail(RSORT_BAD_ARGUMENT, "expert plan arrays overlap");
+    }
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
@@ -792,6 +808,9 @@ rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t typ
     const ByteRange out = rows_range(d_out, p.tokens, out_stride * eb, width * eb);
     if (overlap(rows_range(d_rows, p.rows, rows_stride * eb, width * eb), out))
         return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the rows");
+    const size_t wb = real_bytes(weight_type), slots = size_t(p.tokens) * p.top_k;
+    if (d_weights && overlap(rows_range(d_weights, slots, wb, wb), out))
+        return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the weights");
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
@@ -864,10 +883,16 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
              overlap(out, rows_range(d_rows, p.rows, rows_stride * eb, width * eb))))
             return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
     }
-    const size_t slots = size_t(p.tokens) * p.top_k;
-    if (d_grad_weights && d_weights &&
-        overlap(rows_range(d_grad_weights, slots, wb, wb), rows_range(d_weights, slots, wb, wb)))
-        return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap the weights");
+    if (d_grad_weights) {
+        const size_t slots = size_t(p.tokens) * p.top_k;
+        const ByteRange out = rows_range(d_grad_weights, slots, wb, wb);
+        if (overlap(out, rows_range(d_grad_out, p.tokens, grad_out_stride * eb, width * eb)) ||
+            (d_weights && overlap(out, rows_range(d_weights, slots, wb, wb))) ||
+            (d_rows && overlap(out, rows_range(d_rows, p.rows, rows_stride * eb, width * eb))) ||
+            (d_grad_rows &&
+             overlap(out, rows_range(d_grad_rows, p.rows, grad_rows_stride * eb, width * eb))))
+            return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap another buffer");
+    }
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;

@@ -85,8 +85,8 @@ def device_expert_plan(launch: Launch, tokens: int, top_k: int, experts: int,
     """The plan and the sort's scratch for tokens x top_k slots, with every
     expert's segment padded to a multiple of `align` rows.  Reused from call to
     call, one call at a time."""
-    if tokens < 0 or top_k < 1:
-        raise BadArgument(f"{tokens} tokens, top_k {top_k}")
+    if tokens < 0 or not 1 <= top_k <= _lib.MAX_EXPERTS:
+        raise BadArgument(f"{tokens} tokens, top_k {top_k} (1..{_lib.MAX_EXPERTS})")
     rows = expert_rows(tokens, top_k, experts, align)
     lib = _lib.lib()
     nbytes = lib.rsort_expert_sort_scratch_bytes(tokens * top_k, experts)

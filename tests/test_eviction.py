@@ -59,7 +59,8 @@ def select_status(**kw):
     (dict(scores=None), BAD), (dict(kept=None), BAD), (dict(kept_lengths=None), BAD),
     (dict(budget=0), BAD), (dict(budget=2**31), BAD), (dict(sinks=17), BAD),
     (dict(sinks=13), BAD), (dict(recent=2**64 - 1), BAD), (dict(kept_lengths=0x1000), BAD),
-    (dict(kept_lengths=0x1004), BAD), (dict(scores=0x10002), BAD), (dict(kept=0x2001), BAD),
+    (dict(kept_lengths=0x1004), BAD), (dict(kept=0x10040), BAD), (dict(kept_lengths=0x10000), BAD),
+    (dict(kept=0x0ff8), BAD), (dict(kept_lengths=0x2010), BAD), (dict(scores=0x10002), BAD), (dict(kept=0x2001), BAD),
     (dict(batch=70000), OVERFLOW), (dict(sb=1 << 60), OVERFLOW),
     (dict(capacity=2**31), OVERFLOW)])
 def test_select_refusals(change, status):

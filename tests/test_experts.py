@@ -73,6 +73,11 @@ def sort_status(**kw):
     (dict(t=_lib.RSORT_I64, ids=0x1004), _lib.RSORT_BAD_ARGUMENT),
     (dict(row=0x2001), _lib.RSORT_BAD_ARGUMENT),
     (dict(scratch=0x6002), _lib.RSORT_BAD_ARGUMENT),
+    (dict(row=0x1000), _lib.RSORT_BAD_ARGUMENT),           # over the ids
+    (dict(slot=0x1010), _lib.RSORT_BAD_ARGUMENT),
+    (dict(slot=0x2010), _lib.RSORT_BAD_ARGUMENT),          # over one another
+    (dict(counts=0x4008), _lib.RSORT_BAD_ARGUMENT),
+    (dict(scratch=0x3010), _lib.RSORT_BAD_ARGUMENT),
     (dict(scratch=0x6008), _lib.RSORT_BAD_ARGUMENT)])
 def test_sort_refusals(change, status):
     assert sort_status(**change) == status
@@ -93,6 +98,7 @@ def plan_args(**kw):
     (dict(experts=0), _lib.RSORT_BAD_ARGUMENT),
     (dict(experts=1025), _lib.RSORT_BAD_ARGUMENT),
     (dict(top_k=0), _lib.RSORT_BAD_ARGUMENT),
+    (dict(top_k=1025), _lib.RSORT_BAD_ARGUMENT),
     (dict(tokens=2**31), _lib.RSORT_SIZE_OVERFLOW),
     (dict(nrows=2**31), _lib.RSORT_SIZE_OVERFLOW),
     (dict(offsets=0x2002), _lib.RSORT_BAD_ARGUMENT)])
@@ -139,6 +145,7 @@ F32, F16 = _lib.RSORT_F32, _lib.RSORT_F16
     (F32, 0x10000, 16, 0x20000, F32, 0x30000, 15, 16),              # rows overlap
     (F32, 0x10002, 16, 0x20000, F32, 0x30000, 16, 16),              # alignment
     (F32, 0x10000, 16, 0x20002, F32, 0x30000, 16, 16),
+    (F32, 0x10000, 16, 0x30000, F32, 0x30010, 16, 16),              # output over the weights
     (F16, 0x10000, 16, 0x20000, F32, 0x10010, 16, 16)])             # output over the rows
 def test_combine_refusals(args):
     assert L.rsort_expert_combine(plan_args(), *args, None) == _lib.RSORT_BAD_ARGUMENT
@@ -153,7 +160,10 @@ def test_combine_refusals(args):
     (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x40000, 8, 0x50000, 16),
     (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x40002, 16, 0x50000, 16),
     (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x20000, 16, 0x50000, 16),  # in place
-    (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x40000, 16, 0x30004, 16)])
+    (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x40000, 16, 0x30004, 16),
+    (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, 0x40000, 16, 0x40010, 16),
+    (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, None, 0, 0x20010, 16),
+    (F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, None, 0, 0x10010, 16)])
 def test_combine_backward_refusals(args):
     assert L.rsort_expert_combine_backward(plan_args(), *args, 1, None) == _lib.RSORT_BAD_ARGUMENT
 
@@ -202,5 +212,6 @@ def test_python_refusals():
         experts.device_expert_gather(cub.Launch(torch.device("cuda:0"), Stream()), x, plan, rows)
     with pytest.raises(BadArgument):
         experts.device_expert_plan(CPU, -1, 2, 4)
-    with pytest.raises(BadArgument):
-        experts.device_expert_plan(CPU, 4, 0, 4)
+    for top_k in (0, 1025):
+        with pytest.raises(BadArgument):
+            experts.device_expert_plan(CPU, 4, top_k, 4)

@@ -251,6 +251,26 @@ def test_padding_rows_stay_without_zero_padding():
     assert (grad_rows[s.slot_of_row < 0] == 33).all()
 
 
+@pytest.mark.parametrize("top_k,width", [(3, 8), (3, 2056), (9, 33)])
+def test_dropped_slots_count_for_nothing(top_k, width):
+    """Weights of dropped slots are NaN and the gradient is not finite: what is
+    dropped stays out of the sums and has the gradient 0."""
+    s = Step(21, 40, top_k, 6, 4, width, torch.bfloat16, torch.float32)
+    dropped = torch.from_numpy(s.row_of_slot < 0).view(40, top_k).cuda()
+    assert dropped.any() and not dropped.all()
+    s.w[dropped] = float("nan")
+    y = s.out(40)
+    experts.device_expert_combine(s.lau, s.rows, s.w, s.plan, y)
+    want, mag = combined(s.row_of_slot, s.rows64, s.w64, 40, top_k, width)
+    close(y, want, mag, top_k, torch.bfloat16)
+    s.grad[:, 0] = float("inf")
+    s.grad[:, width - 1] = float("nan")
+    grad_w = torch.full_like(s.w, 44)
+    experts.device_expert_combine_backward(s.lau, s.grad, s.rows, s.w, s.plan, None, grad_w)
+    assert (grad_w[dropped] == 0).all()
+    assert torch.isnan(grad_w[~dropped]).all()
+
+
 def test_gradients_against_differences():
     """The combine is linear in the weights and in the rows, so a difference
     over any step is the gradient but for roundings: 2 * (top_k + 1) roundings
