@@ -4,6 +4,7 @@
 //
 // A cache holds `capacity` positions for each of batch x heads rows; the first
 // lengths[b] of them are in use.
+#include <algorithm>
 #include <climits>
 
 #include "../../include/rsort_b200.h"
@@ -193,13 +194,14 @@ __global__ void __launch_bounds__(ADD_BLOCK, 4) weight_add_kernel(const AddArgs 
 // Selection
 //
 // One cluster of CTAs a head.  Each CTA holds the order images of its slice of
-// the head's totals in registers (totals are read once; only what a slice has
-// beyond SELECT_PAGE is read again), and radix selection finds the
+// the head's totals in registers and, behind SELECT_PAGE of them, in shared
+// memory (only what a slice has beyond three pages is read more than once), and
+// radix selection finds the
 // smallest kept image in three passes of 11, 11 and 10 bits: a pass counts the
 // digits of the images that still match, and every CTA adds up the cluster's
 // counts through distributed shared memory: 64 sums of 32 bins first, then the
 // one sum's bins (every bin of every CTA took 64 us for 64 heads of 64 Ki
-// positions in clusters of eight, bound by that memory; now 25).  Then a count
+// positions in clusters of eight, bound by that memory; so 25).  Then a count
 // of the larger and of the equal images of the CTAs and threads before gives
 // every kept position its place, and a page's positions are put in order in shared memory and written
 // out together.  When every image of the found bin stays, the passes below are
@@ -212,12 +214,13 @@ constexpr uint32_t SELECT_BINS = 4 * SELECT_BLOCK;
 constexpr uint32_t SELECT_MAX_CLUSTER = 8;
 constexpr uint32_t SELECT_ITEMS = 16;  // images a thread holds
 constexpr uint32_t SELECT_PAGE = SELECT_ITEMS * SELECT_BLOCK;
+constexpr uint32_t SELECT_KEPT_PAGES = 2;  // in shared memory, at two CTAs an SM
 
 struct SelectArgs {
     const float *scores;
     size_t score_b, score_h;
     const int32_t *lengths;
-    uint32_t heads, capacity, budget, sinks, recent, cluster;
+    uint32_t heads, capacity, budget, sinks, recent, cluster, kept_pages;
     int32_t *kept, *kept_lengths;
 };
 
@@ -286,12 +289,21 @@ __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const Select
     const uint32_t lo = min(rank * per, m), len = min(per, m - lo);
     const uint32_t pages = (len + SELECT_PAGE - 1) / SELECT_PAGE;
     using Items = uint32_t[SELECT_ITEMS];
-    auto load = [&](uint32_t page, Items &v) {  // item k: position k * SELECT_BLOCK + tid
+    // Item k: position k * SELECT_BLOCK + tid of the page.  Pages behind the first
+    // stay in shared memory, as far as it holds them, each thread's own items.
+    extern __shared__ uint32_t select_kept_pages[];
+    auto load = [&](uint32_t page, Items &v) {
 #pragma unroll
         for (uint32_t k = 0; k < SELECT_ITEMS; ++k) {
             const uint32_t i = page * SELECT_PAGE + k * SELECT_BLOCK + tid;
             v[k] = i < len ? score_image(scores[lo + i]) : 0;
         }
+    };
+    auto load_again = [&](uint32_t page, Items &v) {
+        if (page > a.kept_pages) return load(page, v);
+        const uint32_t *const from = select_kept_pages + (page - 1) * SELECT_PAGE + tid;
+#pragma unroll
+        for (uint32_t k = 0; k < SELECT_ITEMS; ++k) v[k] = from[k * SELECT_BLOCK];
     };
     auto turn = [&](Items &v) {  // item k: position tid * SELECT_ITEMS + k
 #pragma unroll
@@ -327,7 +339,16 @@ __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const Select
         count(held);
         for (uint32_t page = 1; page < pages; ++page) {
             Items v;
-            load(page, v);
+            if (pass == 0) {
+                load(page, v);
+                if (page <= a.kept_pages) {
+                    uint32_t *const to = select_kept_pages + (page - 1) * SELECT_PAGE + tid;
+#pragma unroll
+                    for (uint32_t k = 0; k < SELECT_ITEMS; ++k) to[k * SELECT_BLOCK] = v[k];
+                }
+            } else {
+                load_again(page, v);
+            }
             count(v);
         }
         // This CTA's sums of 32 neighbouring bins: eight threads with four
@@ -387,7 +408,7 @@ __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const Select
     uint32_t larger = total & 0xffff, equal = total >> 16;  // the CTA's
     for (uint32_t page = 1; page < pages; ++page) {
         Items v;
-        load(page, v);
+        load_again(page, v);
         uint32_t sum;
         __syncthreads();
         select_scan(tally(v), warp_sums[1], &sum);
@@ -432,7 +453,7 @@ __global__ void __launch_bounds__(SELECT_BLOCK) cache_select_kernel(const Select
     place(0, held);
     for (uint32_t page = 1; page < pages; ++page) {
         Items v;
-        load(page, v);
+        load_again(page, v);
         __syncthreads();  // the page before has been written
         turn(v);
         before = select_scan(tally(v), warp_sums[0], &total);
@@ -484,7 +505,9 @@ struct Walk {
 };
 
 // Out of place: a CTA moves MOVE_BLOCK * MOVE_UNITS accesses; positions that
-// cannot be read do not move.
+// cannot be read do not move.  (64 heads to 2048 rows of 256 bytes, keys and
+// values, 139 MB: 18.5 us, 31 us with four accesses a thread and divisions by the
+// row's length for each.)
 template <typename U>
 __device__ __forceinline__ void move_out(const Rows &r, const int32_t *kept, const char *src,
                                          char *dst, uint32_t n, uint32_t capacity, uint32_t block) {
@@ -617,8 +640,9 @@ __global__ void __launch_bounds__(MOVE_BLOCK) cache_move_kernel(const __grid_con
 
 // CTAs of a head: enough to hold its totals in registers, as long as all heads
 // run at once (two CTAs an SM).  A CTA costs about 9 us however short its slice:
-// 64 heads of 64 Ki positions take 38 / 25 / 25 us on 2 / 4 / 8 CTAs each (eight
-// need a second wave), 512 heads of 8 Ki 17 / 37 / 76 us on 1 / 2 / 4.
+// 64 heads of 64 Ki positions took 38 / 25 / 25 us on 2 / 4 / 8 CTAs each (eight
+// need a second wave; 22.5 us on 4 with the second page in shared memory), 512
+// heads of 8 Ki take 17 / 37 / 76 us on 1 / 2 / 4.
 uint32_t select_cluster(uint32_t rows, uint32_t capacity, uint32_t sms) {
     uint32_t c = 1;
     while (c < SELECT_MAX_CLUSTER && capacity / c > SELECT_PAGE && rows * c <= sms) c *= 2;
@@ -805,12 +829,25 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
     if (st != RSORT_OK) return st;
     const uint32_t rows = uint32_t(batch * heads);
     const uint32_t cluster = select_cluster(rows, uint32_t(capacity), uint32_t(sms));
+    const uint32_t slice = uint32_t((capacity + cluster - 1) / cluster);
+    const uint32_t kept_pages =
+        slice <= SELECT_PAGE
+            ? 0
+            : std::min((slice + SELECT_PAGE - 1) / SELECT_PAGE - 1, SELECT_KEPT_PAGES);
     SelectArgs a{d_scores,           score_stride_b,  score_stride_h,  d_lengths,
                  uint32_t(heads),    uint32_t(capacity), uint32_t(budget), uint32_t(sinks),
-                 uint32_t(recent),   cluster,         d_kept,          d_kept_lengths};
+                 uint32_t(recent),   cluster,         kept_pages,      d_kept,
+                 d_kept_lengths};
+    const size_t shared = size_t(kept_pages) * SELECT_PAGE * sizeof(uint32_t);
+    if (shared) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(cache_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(SELECT_KEPT_PAGES * SELECT_PAGE * sizeof(uint32_t)));
+        if (e != cudaSuccess) return launched(e, "cache selection shared memory");
+    }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     LaunchScope scope(RSORT_KERNEL_CACHE, s);
-    return launched(launch_early(cache_select_kernel, dim3(rows * cluster), SELECT_BLOCK, 0, cluster,
+    return launched(launch_early(cache_select_kernel, dim3(rows * cluster), SELECT_BLOCK, shared, cluster,
                                  s, a),
                     "cache selection launch");
 }

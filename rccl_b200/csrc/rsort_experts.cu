@@ -28,6 +28,10 @@ namespace {
 //     another's counts through distributed shared memory.
 //   longer: a first kernel counts the experts of every CTA's chunk, the second
 //     adds up the chunks before its own; it starts early and ranks meanwhile.
+// 128 slots take 4.1 us, 2 Ki 5.4, 8 Ki 5.5, 32 Ki 9.2, 512 Ki 13 (both launches).
+// In a full CTA of 4096 slots and 256 experts a quarter of the time goes to the
+// votes (33 cycles of the SM for 32 slots) and a quarter to the scattered stores
+// of slot_of_row (35 cycles).
 // ---------------------------------------------------------------------------
 constexpr uint32_t SORT_STEPS = 4;
 constexpr uint32_t SORT_MAX_WARPS = 32;
@@ -334,6 +338,10 @@ __device__ __forceinline__ void zero_padding(const Plan &p, uint32_t b, char *ro
     }
 }
 
+// rows[row of slot] = x[t]: a token is read once and written to all of its rows,
+// so the kernel is bound by the writes (16 Ki tokens to 8 rows of 4096 bf16 and
+// the padding of 128 experts, 1.27 GB, 205 us: 6.2 TB/s; 8191 tokens to 6 rows
+// of 2048, 240 MB, 36 us: 6.6 TB/s).
 template <typename U>
 __global__ void __launch_bounds__(ROW_BLOCK)
     expert_gather_kernel(const Plan p, const Shape s, const char *x, size_t x_stride, char *rows,

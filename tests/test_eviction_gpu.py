@@ -146,6 +146,23 @@ def test_select(H, S, budget, sinks, recent, lens, kind):
     assert np.array_equal(n.cpu().numpy(), want_n)
 
 
+@pytest.mark.parametrize("kind", ["ties", "close", "heavy"])
+@pytest.mark.parametrize("B,S,budget", [(1, 300_000, 20_000), (170, 9000, 500), (150, 33_000, 32_990)])
+def test_select_over_many_pages(B, S, budget, kind):
+    """Slices beyond what a CTA holds in registers and in shared memory, and more
+    heads than run at once."""
+    rng = np.random.default_rng(S)
+    scores = make_scores(rng, kind, (B, 1, S))
+    lens = [S] + [int(x) for x in rng.integers(budget, S + 1, B - 1)]
+    kept = torch.zeros(B, 1, budget, dtype=torch.int32, device="cuda")
+    n = torch.zeros(B, dtype=torch.int32, device="cuda")
+    eviction.device_cache_select(launch(), torch.from_numpy(scores).cuda(), lengths_of(lens), kept,
+                                 n, 3, 5)
+    want, want_n = selected(scores, lens, budget, 3, 5)
+    assert np.array_equal(kept.cpu().numpy(), want)
+    assert np.array_equal(n.cpu().numpy(), want_n)
+
+
 def test_select_without_lengths_and_clamped():
     rng = np.random.default_rng(9)
     scores = make_scores(rng, "heavy", (3, 2, 200))
