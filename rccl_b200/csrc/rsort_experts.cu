@@ -27,8 +27,10 @@ namespace {
 //   up to SORT_MAX_CLUSTER CTAs: one launch of one cluster; its CTAs read one
 //     another's counts through distributed shared memory.
 //   longer: a first kernel counts the experts of every CTA's chunk, the second
-//     adds up the chunks before its own; it starts early and ranks meanwhile.
-// 128 slots take 4.1 us, 2 Ki 5.4, 8 Ki 5.5, 32 Ki 9.2, 512 Ki 13 (both launches).
+//     adds up the chunks before its own.  The second comes onto the SMs early,
+//     but reads no ids before it has waited itself: that the first has waited
+//     for whoever wrote the ids shows them to the first alone.
+// 128 slots take 4.1 us, 2 Ki 5.4, 8 Ki 5.5, 32 Ki 9.2, 512 Ki 14.5 (both launches).
 // In a full CTA of 4096 slots and 256 experts a quarter of the time goes to the
 // votes (33 cycles of the SM for 32 slots) and a quarter to the scattered stores
 // of slot_of_row (35 cycles).
@@ -134,21 +136,19 @@ __global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_place_kernel(const
     const uint64_t end = min(begin + a.chunk, uint64_t(a.n));
     const uint32_t part = SORT_STEPS * blockDim.x;  // slots taken at once
 
-    // With a counting kernel before it, this one ranks its slots meanwhile:
-    // that kernel waited for what came before.
-    if (!a.counts_of_block) begin_kernel();
     for (uint64_t p = begin; p == begin || p < end; p += part) {
         const uint64_t slot0 = p + uint64_t(warp) * (SORT_STEPS * 32) + lane;
         uint32_t e[SORT_STEPS], rank[SORT_STEPS];
-#pragma unroll
-        for (uint32_t k = 0; k < SORT_STEPS; ++k)
-            e[k] = slot0 + 32 * k < end ? bucket<I>(a, slot0 + 32 * k) : E;
         for (uint32_t i = tid; i < warps * pitch / 2; i += blockDim.x)
             reinterpret_cast<uint32_t *>(base)[i] = 0;
         if (p == begin) {
             for (uint32_t i = tid; i < E; i += blockDim.x) total[i] = first[i] = 0;
+            begin_kernel();
             if (!a.counts_of_block) clear_rows(a);
         }
+#pragma unroll
+        for (uint32_t k = 0; k < SORT_STEPS; ++k)
+            e[k] = slot0 + 32 * k < end ? bucket<I>(a, slot0 + 32 * k) : E;
         __syncthreads();
         // Ranks among the warp's slots: lanes with the same expert in lane
         // order, step after step.
@@ -181,7 +181,6 @@ __global__ void __launch_bounds__(SORT_MAX_WARPS * 32) expert_place_kernel(const
         if (p == begin) {
             // The experts' totals and the slots of the CTAs before this one.
             if (a.counts_of_block) {
-                begin_kernel();
                 const uint32_t quads = a.pitch / 4, wide = (quads + 31) & ~31u;
                 const uint32_t groups = max(blockDim.x / wide, 1u);
                 const uint4 *const counts = reinterpret_cast<const uint4 *>(a.counts_of_block);

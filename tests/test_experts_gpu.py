@@ -374,3 +374,66 @@ def test_calls_count_as_launches_of_this_library():
     lib.rsort_launch_count_reset()
     experts.device_expert_combine(s.lau, s.rows, s.w, s.plan, s.out(8))
     assert lib.rsort_launch_count() == 1
+
+
+def long_ids(seed, tokens, top_k, count):
+    """Ids of a sort of more than one cluster, a third of them dropped."""
+    return make_ids(np.random.default_rng(seed), tokens, top_k, count, "mixed", torch.int64)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_long_sort_of_ids_that_a_kernel_has_just_written(dtype):
+    """The ids' kernel and both kernels of the sort follow one another closely,
+    over and over into the same buffers: every plan is that of its own ids."""
+    tokens, top_k, count, align = 50_001, 3, 96, 8
+    lau = launch()
+    plan = experts.device_expert_plan(lau, tokens, top_k, count, align)
+    drawn = [long_ids(seed, tokens, top_k, count) for seed in range(8)]
+    drawn = [ids.clamp(-1, count).to(dtype) for ids in drawn]
+    on_device = [ids.cuda() for ids in drawn]
+    ids = torch.full((tokens, top_k), -1, dtype=dtype, device="cuda")
+    seen = []
+    torch.cuda.synchronize()
+    for source in on_device:
+        torch.add(source, 0, out=ids)
+        experts.device_expert_sort(lau, ids, plan)
+        seen.append([t.clone() for t in (plan.row_of_slot, plan.slot_of_row, plan.offsets,
+                                         plan.counts)])
+    for source, got in zip(drawn, seen):
+        want = sorted_plan(source.reshape(-1).numpy().astype(np.int64), count, align)
+        for w, g in zip(want, got):
+            assert np.array_equal(g.view(-1).cpu().numpy().astype(np.int64), w)
+
+
+def test_long_sort_captured_behind_the_kernel_of_its_ids():
+    """The form of two launches as part of a replayed graph, twice in a row."""
+    tokens, top_k, count, align = 40_003, 4, 60, 16
+    program = cub.Program.load("cuda:0")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lau = program.on(side)
+        plans = [experts.device_expert_plan(lau, tokens, top_k, count, align) for _ in range(2)]
+        source = torch.zeros(tokens, top_k, dtype=torch.int64, device="cuda")
+        ids = torch.zeros_like(source)
+
+    def run(on):
+        torch.add(source, 0, out=ids)
+        experts.device_expert_sort(on, ids, plans[0])
+        torch.add(source, 1, out=ids)
+        experts.device_expert_sort(on, ids, plans[1])
+
+    with torch.cuda.stream(side):
+        run(lau)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run(program.on(torch.cuda.current_stream()))
+    for seed in range(3):
+        drawn = long_ids(seed, tokens, top_k, count).clamp(-2, count)
+        with torch.cuda.stream(side):
+            source.copy_(drawn)
+            graph.replay()
+        side.synchronize()
+        check_plan(plans[0], drawn, count, align)
+        check_plan(plans[1], drawn + 1, count, align)
