@@ -658,74 +658,6 @@ rsort_status check_grid(size_t batch, size_t heads, size_t capacity) {
     return RSORT_OK;
 }
 
-// A strided [batch, heads, positions] array of `bytes`-wide items; strides in
-// bytes, dimensions of one entry dropped, smallest stride first.
-struct Strided {
-    uintptr_t base;
-    size_t bytes;
-    size_t stride[3], count[3];
-    int dims;
-    ByteRange range;
-};
-
-// False when an offset could wrap.
-bool strided(const void *p, size_t batch, size_t heads, size_t n, size_t sb, size_t sh, size_t ss,
-             size_t bytes, Strided *out) {
-    if (!rows_fit(batch, sb, bytes) || !rows_fit(heads, sh, bytes) || !rows_fit(n, ss, bytes))
-        return false;
-    const size_t stride[3] = {ss, sh, sb}, count[3] = {n, heads, batch};
-    Strided r{addr(p), bytes, {}, {}, 0, {}};
-    size_t extent = bytes;
-    for (int i = 0; i < 3; ++i) {
-        if (count[i] <= 1) continue;
-        int at = r.dims++;
-        for (; at > 0 && r.stride[at - 1] > stride[i]; --at) {
-            r.stride[at] = r.stride[at - 1];
-            r.count[at] = r.count[at - 1];
-        }
-        r.stride[at] = stride[i];
-        r.count[at] = count[i];
-        extent += (count[i] - 1) * stride[i];
-    }
-    r.range = {r.base, r.base + extent};
-    *out = r;
-    return true;
-}
-
-// No two items share a byte (sufficient: every stride spans what lies inside).
-bool items_apart(const Strided &a) {
-    size_t inner = a.bytes;
-    for (int i = 0; i < a.dims; ++i) {
-        if (a.stride[i] < inner) return false;
-        inner += (a.count[i] - 1) * a.stride[i];
-    }
-    return true;
-}
-
-// No item of one shares a byte with an item of the other (sufficient: their
-// ranges are apart, or both have the same strides and interleave, as the keys
-// and values of one packed allocation do).
-bool arrays_apart(const Strided &a, const Strided &b) {
-    if (!overlap(a.range, b.range)) return true;
-    if (a.dims != b.dims || a.bytes != b.bytes) return false;
-    for (int i = 0; i < a.dims; ++i)
-        if (a.stride[i] != b.stride[i]) return false;
-    const size_t d = a.base < b.base ? b.base - a.base : a.base - b.base;
-    size_t inner = a.bytes;
-    for (int i = 0; i < a.dims; ++i) {
-        // Everything below dimension i lies within `inner` bytes of a multiple
-        // of its stride when the larger strides are multiples of it too.
-        bool multiples = a.stride[i] > 0;
-        for (int j = i + 1; j < a.dims && multiples; ++j) multiples = a.stride[j] % a.stride[i] == 0;
-        if (multiples) {
-            const size_t r = d % a.stride[i];
-            if (r >= inner && r + inner <= a.stride[i]) return true;
-        }
-        inner += ((a.count[i] > b.count[i] ? a.count[i] : b.count[i]) - 1) * a.stride[i];
-    }
-    return false;
-}
-
 }  // namespace
 
 extern "C" {
@@ -750,7 +682,7 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
         !rows_fit(heads * group, stride_h * eb, 0) || !rows_fit(queries, stride_q * eb, 0))
         return fail(RSORT_SIZE_OVERFLOW, "attention weight strides");
     Strided scores{};
-    if (!strided(d_scores, batch, heads, capacity, score_stride_b * 4, score_stride_h * 4, 4, 4,
+    if (!strided(d_scores, 4, {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}},
                  &scores))
         return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
     if (!items_apart(scores)) return fail(RSORT_BAD_ARGUMENT, "cache score strides overlap");
@@ -811,18 +743,17 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
     st = check_alignment(addr(d_scores) | addr(d_lengths) | addr(d_kept) | addr(d_kept_lengths), 4,
                          "cache selection alignment");
     if (st != RSORT_OK) return st;
-    if (d_lengths &&
-        overlap(rows_range(d_kept_lengths, batch, 4, 4), rows_range(d_lengths, batch, 4, 4)))
+    const Strided kept = packed(d_kept, batch * heads * budget * 4);
+    const Strided kept_n = packed(d_kept_lengths, batch * 4);
+    const Strided lengths = packed(d_lengths, d_lengths ? batch * 4 : 0);
+    if (!apart(kept_n, lengths))
         return fail(RSORT_BAD_ARGUMENT, "kept lengths overlap the lengths");
     Strided scores{};
-    if (!strided(d_scores, batch, heads, capacity, score_stride_b * 4, score_stride_h * 4, 4, 4,
+    if (!strided(d_scores, 4, {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}},
                  &scores))
         return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
-    const ByteRange kept = rows_range(d_kept, batch * heads * budget, 4, 4);
-    const ByteRange kept_n = rows_range(d_kept_lengths, batch, 4, 4);
-    const ByteRange read = capacity ? scores.range : ByteRange{0, 0};
-    if (overlap(kept, read) || overlap(kept_n, read) || overlap(kept, kept_n) ||
-        (d_lengths && overlap(kept, rows_range(d_lengths, batch, 4, 4))))
+    if (!apart(kept, scores) || !apart(kept_n, scores) || !apart(kept, kept_n) ||
+        !apart(kept, lengths))
         return fail(RSORT_BAD_ARGUMENT, "kept positions overlap another buffer");
     int sms = 0;
     st = current_sm_count(&sms);
@@ -866,8 +797,7 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
     st = check_alignment(addr(d_kept) | addr(d_kept_lengths), 4, "cache selection alignment");
     if (st != RSORT_OK) return st;
     const size_t bh = batch * heads;
-    const ByteRange kept = rows_range(d_kept, bh * budget, 4, 4);
-    const ByteRange kept_n = rows_range(d_kept_lengths, batch, 4, 4);
+    const Strided kept = packed(d_kept, bh * budget * 4), kept_n = packed(d_kept_lengths, batch * 4);
     Strided in[RSORT_MAX_CACHES], out[RSORT_MAX_CACHES];
     bool in_place = false;
     for (size_t i = 0; i < ncaches; ++i) {
@@ -882,19 +812,22 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
         if (same && (c.src_stride_b != c.dst_stride_b || c.src_stride_h != c.dst_stride_h ||
                      c.src_stride_s != c.dst_stride_s))
             return fail(RSORT_BAD_ARGUMENT, "cache strides in place");
-        if (!strided(c.src, batch, heads, capacity, c.src_stride_b, c.src_stride_h, c.src_stride_s,
-                     c.row_bytes, &in[i]) ||
-            !strided(c.dst, batch, heads, same || budget > capacity ? capacity : budget,
-                     c.dst_stride_b, c.dst_stride_h, c.dst_stride_s, c.row_bytes, &out[i]))
+        const size_t written = same || budget > capacity ? capacity : budget;
+        if (!strided(c.src, c.row_bytes,
+                     {{capacity, c.src_stride_s}, {heads, c.src_stride_h}, {batch, c.src_stride_b}},
+                     &in[i]) ||
+            !strided(c.dst, c.row_bytes,
+                     {{written, c.dst_stride_s}, {heads, c.dst_stride_h}, {batch, c.dst_stride_b}},
+                     &out[i]))
             return fail(RSORT_SIZE_OVERFLOW, "cache strides");
         if (!items_apart(out[i])) return fail(RSORT_BAD_ARGUMENT, "cache strides overlap");
-        if (overlap(out[i].range, kept) || overlap(out[i].range, kept_n))
+        if (!apart(out[i], kept) || !apart(out[i], kept_n))
             return fail(RSORT_BAD_ARGUMENT, "caches overlap the kept positions");
     }
     for (size_t i = 0; i < ncaches; ++i)
         for (size_t j = 0; j < ncaches; ++j)
-            if ((i != j && !arrays_apart(out[i], out[j])) ||
-                ((i != j || !in_place) && !arrays_apart(out[i], in[j])))
+            if ((i != j && !apart(out[i], out[j])) ||
+                ((i != j || !in_place) && !apart(out[i], in[j])))
                 return fail(RSORT_BAD_ARGUMENT, "caches overlap");
     int sms = 0;
     st = current_sm_count(&sms);

@@ -707,16 +707,14 @@ rsort_status rsort_expert_sort(rsort_key_t id_type, const void *d_ids, size_t ns
     if (st == RSORT_OK) st = check_alignment(addr(d_scratch), 16, "expert sort scratch alignment");
     if (st != RSORT_OK) return st;
     const size_t id_bytes = id_type == RSORT_I64 ? 8 : 4;
-    const ByteRange ids = rows_range(d_ids, nslots, id_bytes, id_bytes);
-    const ByteRange written[] = {rows_range(d_row_of_slot, nslots, 4, 4),
-                                 rows_range(d_slot_of_row, nrows, 4, 4),
-                                 rows_range(d_offsets, experts + 1, 4, 4),
-                                 rows_range(d_counts, experts, 4, 4),
-                                 rows_range(d_scratch, bytes, 1, 1)};
-    for (const ByteRange &w : written) {
-        if (overlap(ids, w)) return fail(RSORT_BAD_ARGUMENT, "expert plan overlaps the ids");
-        for (const ByteRange &v : written)
-            if (&v != &w && overlap(v, w))
+    const Strided ids = packed(d_ids, nslots * id_bytes);
+    const Strided written[] = {packed(d_row_of_slot, nslots * 4), packed(d_slot_of_row, nrows * 4),
+                               packed(d_offsets, (experts + 1) * 4), packed(d_counts, experts * 4),
+                               packed(d_scratch, bytes)};
+    for (const Strided &w : written) {
+        if (!apart(ids, w)) return fail(RSORT_BAD_ARGUMENT, "expert plan overlaps the ids");
+        for (const Strided &v : written)
+            if (&v != &w && !apart(v, w))
                 return fail(RSORT_BAD_ARGUMENT, "expert plan arrays overlap");
     }
     int sms = 0;
@@ -760,10 +758,11 @@ rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x,
     if ((p.tokens && !d_x) || !d_rows) return fail(RSORT_BAD_ARGUMENT, "null buffer");
     if (p.rows > 1 && rows_stride < row_bytes)
         return fail(RSORT_BAD_ARGUMENT, "expert rows stride", row_bytes, rows_stride);
-    if (!rows_fit(p.tokens, x_stride, row_bytes) || !rows_fit(p.rows, rows_stride, row_bytes))
+    Strided x, rows;
+    if (!strided(d_x, row_bytes, {{p.tokens, x_stride}}, &x) ||
+        !strided(d_rows, row_bytes, {{p.rows, rows_stride}}, &rows))
         return fail(RSORT_SIZE_OVERFLOW, "expert rows");
-    if (overlap(rows_range(d_x, p.tokens, x_stride, row_bytes),
-                rows_range(d_rows, p.rows, rows_stride, row_bytes)))
+    if (!apart(x, rows))
         return fail(RSORT_BAD_ARGUMENT, "expert rows overlap the tokens");
     int sms = 0;
     st = current_sm_count(&sms);
@@ -805,18 +804,18 @@ rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t typ
     if (p.tokens > 1 && out_stride < width)
         return fail(RSORT_BAD_ARGUMENT, "expert output stride", width, out_stride);
     constexpr size_t most = size_t(1) << 53;
-    if (rows_stride > most || out_stride > most || !rows_fit(p.rows, rows_stride * eb, width * eb) ||
-        !rows_fit(p.tokens, out_stride * eb, width * eb))
+    Strided rows, out;
+    if (rows_stride > most || out_stride > most ||
+        !strided(d_rows, width * eb, {{p.rows, rows_stride * eb}}, &rows) ||
+        !strided(d_out, width * eb, {{p.tokens, out_stride * eb}}, &out))
         return fail(RSORT_SIZE_OVERFLOW, "expert rows");
     st = check_alignment(addr(d_rows) | addr(d_out), eb, "expert rows alignment");
     if (st == RSORT_OK && d_weights)
         st = check_alignment(addr(d_weights), real_bytes(weight_type), "expert weights alignment");
     if (st != RSORT_OK) return st;
-    const ByteRange out = rows_range(d_out, p.tokens, out_stride * eb, width * eb);
-    if (overlap(rows_range(d_rows, p.rows, rows_stride * eb, width * eb), out))
-        return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the rows");
-    const size_t wb = real_bytes(weight_type), slots = size_t(p.tokens) * p.top_k;
-    if (d_weights && overlap(rows_range(d_weights, slots, wb, wb), out))
+    if (!apart(rows, out)) return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the rows");
+    const size_t weight_bytes = size_t(p.tokens) * p.top_k * real_bytes(weight_type);
+    if (d_weights && !apart(packed(d_weights, weight_bytes), out))
         return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the weights");
     int sms = 0;
     st = current_sm_count(&sms);
@@ -871,10 +870,12 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
     if (d_grad_rows && p.rows > 1 && grad_rows_stride < width)
         return fail(RSORT_BAD_ARGUMENT, "expert gradient rows stride", width, grad_rows_stride);
     constexpr size_t most = size_t(1) << 53;
+    Strided grad_out, rows, grad_rows;
     if (rows_stride > most || grad_out_stride > most || grad_rows_stride > most ||
-        !rows_fit(p.rows, rows_stride * eb, width * eb) ||
-        !rows_fit(p.rows, grad_rows_stride * eb, width * eb) ||
-        !rows_fit(p.tokens, grad_out_stride * eb, width * eb))
+        !strided(d_rows, width * eb, {{d_rows ? p.rows : 0, rows_stride * eb}}, &rows) ||
+        !strided(d_grad_rows, width * eb, {{d_grad_rows ? p.rows : 0, grad_rows_stride * eb}},
+                 &grad_rows) ||
+        !strided(d_grad_out, width * eb, {{p.tokens, grad_out_stride * eb}}, &grad_out))
         return fail(RSORT_SIZE_OVERFLOW, "expert rows");
     st = check_alignment(addr(d_grad_out) | addr(d_rows) | addr(d_grad_rows), eb,
                          "expert rows alignment");
@@ -882,22 +883,14 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
         st = check_alignment(addr(d_weights) | addr(d_grad_weights), wb,
                              "expert weights alignment");
     if (st != RSORT_OK) return st;
-    if (d_grad_rows) {
-        const ByteRange out =
-            rows_range(d_grad_rows, p.rows, grad_rows_stride * eb, width * eb);
-        if (overlap(out, rows_range(d_grad_out, p.tokens, grad_out_stride * eb, width * eb)) ||
-            (d_grad_weights && d_rows &&
-             overlap(out, rows_range(d_rows, p.rows, rows_stride * eb, width * eb))))
-            return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
-    }
+    // Without weight gradients the rows are not read.
+    if (!apart(grad_rows, grad_out) || (d_grad_weights && !apart(grad_rows, rows)))
+        return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
     if (d_grad_weights) {
-        const size_t slots = size_t(p.tokens) * p.top_k;
-        const ByteRange out = rows_range(d_grad_weights, slots, wb, wb);
-        if (overlap(out, rows_range(d_grad_out, p.tokens, grad_out_stride * eb, width * eb)) ||
-            (d_weights && overlap(out, rows_range(d_weights, slots, wb, wb))) ||
-            (d_rows && overlap(out, rows_range(d_rows, p.rows, rows_stride * eb, width * eb))) ||
-            (d_grad_rows &&
-             overlap(out, rows_range(d_grad_rows, p.rows, grad_rows_stride * eb, width * eb))))
+        const size_t weight_bytes = size_t(p.tokens) * p.top_k * wb;
+        const Strided out = packed(d_grad_weights, weight_bytes);
+        if (!apart(out, grad_out) || !apart(out, rows) || !apart(out, grad_rows) ||
+            (d_weights && !apart(out, packed(d_weights, weight_bytes))))
             return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap another buffer");
     }
     int sms = 0;

@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -45,23 +46,89 @@ inline size_t access_bytes(uintptr_t bits, size_t most) {
     return a;
 }
 
-// [first, last) of n rows of `bytes`, `stride` bytes apart.
-struct ByteRange {
-    uintptr_t first, last;
-};
-inline ByteRange rows_range(const void *p, size_t n, size_t stride, size_t bytes) {
-    if (n == 0 || bytes == 0) return {addr(p), addr(p)};
-    return {addr(p), addr(p) + (n - 1) * stride + bytes};
-}
-inline bool overlap(const ByteRange &a, const ByteRange &b) {
-    return a.first < a.last && b.first < b.last && a.first < b.last && b.first < a.last;
-}
-
 // n rows `stride` bytes apart stay below 2^56 bytes, far beyond any device,
 // so no offset of theirs wraps.
 inline bool rows_fit(size_t n, size_t stride, size_t bytes) {
     constexpr size_t kMost = size_t(1) << 56;
     return bytes <= kMost && (n == 0 || stride <= kMost / n);
+}
+
+// An array of `bytes`-wide items along up to four axes, strides in bytes;
+// axes of one entry dropped, smallest stride first.  [first, last) spans it
+// (nothing without items).
+struct Axis {
+    size_t count, stride;
+};
+struct Strided {
+    uintptr_t first = 0, last = 0;
+    size_t bytes = 0;
+    Axis axis[4] = {};
+    int axes = 0;
+};
+
+// False when an offset could wrap.
+inline bool strided(const void *p, size_t bytes, std::initializer_list<Axis> axes, Strided *out) {
+    Strided r;
+    r.first = r.last = addr(p);
+    r.bytes = bytes;
+    size_t extent = bytes;
+    bool empty = bytes == 0;
+    for (const Axis &x : axes) {
+        if (!rows_fit(x.count, x.stride, bytes)) return false;
+        empty |= x.count == 0;
+        if (x.count <= 1) continue;
+        int at = r.axes++;
+        for (; at > 0 && r.axis[at - 1].stride > x.stride; --at) r.axis[at] = r.axis[at - 1];
+        r.axis[at] = x;
+        extent += (x.count - 1) * x.stride;
+    }
+    if (!empty) r.last += extent;
+    *out = r;
+    return true;
+}
+
+// `bytes` next to one another.
+inline Strided packed(const void *p, size_t bytes) {
+    Strided r;
+    strided(p, bytes, {}, &r);
+    return r;
+}
+
+// No two items share a byte (sufficient: every stride spans what lies inside).
+inline bool items_apart(const Strided &a) {
+    size_t inner = a.bytes;
+    for (int i = 0; i < a.axes; ++i) {
+        if (a.axis[i].stride < inner) return false;
+        inner += (a.axis[i].count - 1) * a.axis[i].stride;
+    }
+    return true;
+}
+
+// No item of one shares a byte with an item of the other (sufficient: their
+// spans are apart, or they lie side by side within some stride s of theirs, as
+// keys and values of one allocation do: axes whose strides are multiples of s
+// leave an address as it is modulo s, so each array covers one interval there).
+inline bool apart(const Strided &a, const Strided &b) {
+    if (a.first >= b.last || b.first >= a.last || a.first >= a.last || b.first >= b.last)
+        return true;
+    const auto width = [](const Strided &x, size_t s) {
+        size_t w = x.bytes;
+        for (int i = 0; i < x.axes; ++i)
+            if (x.axis[i].stride % s) w += (x.axis[i].count - 1) * x.axis[i].stride;
+        return w;
+    };
+    const auto side_by_side = [&](size_t s) {
+        if (s == 0) return false;
+        const size_t wa = width(a, s), wb = width(b, s);
+        const size_t d = b.first >= a.first ? (b.first - a.first) % s
+                                            : (s - (a.first - b.first) % s) % s;
+        return wa <= d && wb <= s - d;
+    };
+    for (int i = 0; i < a.axes; ++i)
+        if (side_by_side(a.axis[i].stride)) return true;
+    for (int i = 0; i < b.axes; ++i)
+        if (side_by_side(b.axis[i].stride)) return true;
+    return false;
 }
 
 // Thread-block clusters: a word of CTA `rank`'s shared memory at the same

@@ -158,3 +158,22 @@ def test_python_refusals():
             compact(CPU, *bad)
     with pytest.raises(cub.ContextMismatch):
         compact(cub.Launch(torch.device("cuda:0"), Stream()), kept, n, [k])
+
+
+def test_rows_of_one_allocation_that_share_a_byte_are_refused():
+    """Rows of 64 and 32 bytes in places of 96: apart side by side, refused as
+    soon as they share a byte."""
+    def view(offset, row_bytes, base):
+        return dict(row_bytes=row_bytes, src=base + offset, src_stride_s=96, src_stride_h=64 * 96,
+                    src_stride_b=128 * 96)
+
+    def into(offset, base):
+        return dict(dst=base + offset, dst_stride_s=96, dst_stride_h=64 * 96, dst_stride_b=128 * 96)
+
+    for offset in (63, 65, 1, 95):
+        rows = [cache(**view(0, 64, 0x100000), **into(0, 0x200000)),
+                cache(**view(64, 32, 0x100000), **into(offset, 0x200000))]
+        assert compact_status(*rows) == BAD
+        rows = [cache(**view(0, 64, 0x100000), **into(0, 0x100000)),
+                cache(**view(offset, 32, 0x100000), **into(offset, 0x100000))]
+        assert compact_status(*rows) == BAD

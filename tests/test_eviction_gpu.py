@@ -321,3 +321,36 @@ def test_a_bounded_cache_over_many_tokens(captured):
     assert np.array_equal(scores.cpu().numpy()[:, :, :hl], hs[:, :, :hl])
     rounded = torch.from_numpy(hk[:, :, :hl]).bfloat16()
     assert torch.equal(v.cpu()[:, :, :hl], rounded)
+
+
+def one_allocation(rng, B, S, H, widths):
+    """Keys, values (bf16) and totals (f32) of every position side by side in
+    one allocation: (B, H, S, width) views of unequal widths and the totals."""
+    k_width, v_width = widths
+    block = torch.from_numpy(rng.integers(0, 256, (B, S, H, 2 * (k_width + v_width) + 4),
+                                          dtype=np.uint8)).cuda()
+    k = block[..., :2 * k_width].view(torch.bfloat16).transpose(1, 2)
+    v = block[..., 2 * k_width:-4].view(torch.bfloat16).transpose(1, 2)
+    scores = block[..., -4:].view(torch.float32)[..., 0].transpose(1, 2)
+    return block, [k, v, scores]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("widths", [(64, 8), (16, 48), (5, 3), (2, 2)])
+@pytest.mark.parametrize("H", [1, 3])
+def test_compact_of_unequal_rows_in_one_allocation(H, widths, in_place):
+    """Arrays that interleave without sharing a byte move together, whatever
+    their rows' widths; nothing beside the moved rows changes."""
+    rng = np.random.default_rng(sum(widths) + H)
+    B, S, budget, lens = 2, 90, 31, [90, 40]
+    kept, n = random_kept(rng, B, H, S, budget, lens)
+    block, src = one_allocation(rng, B, S, H, widths)
+    to, dst = (block, src) if in_place else one_allocation(rng, B, budget, H, widths)
+    want = to.clone()
+    for b in range(B):
+        for h in range(H):
+            at = torch.from_numpy(kept[b, h, :n[b]]).long().cuda()
+            want[b, :n[b], h] = block[b, at, h]
+    eviction.device_cache_compact(launch(), torch.from_numpy(kept).cuda(),
+                                  torch.from_numpy(n).cuda(), src, None if in_place else dst)
+    assert torch.equal(to, want)

@@ -437,3 +437,43 @@ def test_long_sort_captured_behind_the_kernel_of_its_ids():
         side.synchronize()
         check_plan(plans[0], drawn, count, align)
         check_plan(plans[1], drawn + 1, count, align)
+
+
+@pytest.mark.parametrize("dtype,width", [(torch.float32, 24), (torch.bfloat16, 72),
+                                         (torch.float16, 7)])
+def test_rows_and_outputs_side_by_side_in_one_allocation(dtype, width):
+    """Inputs and outputs as columns of one buffer: none shares a byte with
+    another, and the columns that no call writes stay."""
+    tokens, top_k, count, align = 40, 3, 5, 4
+    s = Step(31, tokens, top_k, count, align, width, dtype, torch.float32)
+    height = max(s.plan.rows, tokens)
+
+    def columns():
+        both = torch.full((height, 2 * width), 9, dtype=dtype, device="cuda")
+        return both[:, :width], both[:, width:]
+
+    y = s.out(tokens)
+    experts.device_expert_combine(s.lau, s.rows, s.w, s.plan, y)
+    left, right = columns()
+    left[:s.plan.rows].copy_(s.rows)
+    before = left.clone()
+    experts.device_expert_combine(s.lau, left, s.w, s.plan, right[:tokens])
+    assert torch.equal(right[:tokens], y) and (right[tokens:] == 9).all()
+    assert torch.equal(left.nan_to_num(3), before.nan_to_num(3))
+
+    rows = s.out(s.plan.rows)
+    experts.device_expert_gather(s.lau, s.grad, s.plan, rows)
+    left, right = columns()
+    left[:tokens].copy_(s.grad)
+    right[:s.plan.rows].fill_(33)
+    experts.device_expert_gather(s.lau, left[:tokens], s.plan, right)
+    assert torch.equal(right[:s.plan.rows], rows) and torch.equal(left[:tokens], s.grad)
+
+    grad_rows, grad_w = s.out(s.plan.rows), torch.full_like(s.w, 44)
+    experts.device_expert_combine_backward(s.lau, s.grad, s.rows, s.w, s.plan, grad_rows, grad_w)
+    left, right = columns()
+    left[:s.plan.rows].copy_(s.rows)
+    right[:s.plan.rows].fill_(33)
+    got_w = torch.full_like(s.w, 44)
+    experts.device_expert_combine_backward(s.lau, s.grad, left, s.w, s.plan, right, got_w)
+    assert torch.equal(right[:s.plan.rows], grad_rows) and torch.equal(got_w, grad_w)
