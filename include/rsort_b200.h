@@ -592,7 +592,8 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
  *       causal the queries are the last ones of the sequence: query q sees
  *       s <= lengths[b] - queries + q, and what it does not see is not read.
  *       Weights are f32, f16 or bf16; strides in elements, positions next to
- *       one another.  Null lengths: every position is in use.
+ *       one another.  Null lengths: every position is in use.  The totals must
+ *       not share a byte with the weights or the lengths.
  *   rsort_cache_select
  *       kept[b, h, 0..budget-1]: the positions that stay, ascending, then -1;
  *       kept_lengths[b] = min(lengths[b], budget).  A sequence of at most

@@ -677,15 +677,21 @@ rsort_status rsort_attention_weight_add(rsort_key_t type, const void *d_weights,
     if (batch == 0 || heads == 0 || capacity == 0) return RSORT_OK;
     if ((queries && !d_weights) || !d_scores) return fail(RSORT_BAD_ARGUMENT, "null buffer");
     constexpr size_t most = size_t(1) << 50;
+    Strided weights, scores;
     if (stride_b > most || stride_h > most || stride_q > most || score_stride_b > most ||
-        score_stride_h > most || !rows_fit(batch, stride_b * eb, 0) ||
-        !rows_fit(heads * group, stride_h * eb, 0) || !rows_fit(queries, stride_q * eb, 0))
+        score_stride_h > most ||
+        !strided(d_weights, capacity * eb,
+                 {{queries, stride_q * eb}, {heads * group, stride_h * eb}, {batch, stride_b * eb}},
+                 &weights))
         return fail(RSORT_SIZE_OVERFLOW, "attention weight strides");
-    Strided scores{};
-    if (!strided(d_scores, 4, {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}},
-                 &scores))
+    if (!strided(d_scores, 4,
+                 {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}}, &scores))
         return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
     if (!items_apart(scores)) return fail(RSORT_BAD_ARGUMENT, "cache score strides overlap");
+    if (!apart(scores, weights))
+        return fail(RSORT_BAD_ARGUMENT, "cache scores overlap the weights");
+    if (d_lengths && !apart(scores, packed(d_lengths, batch * 4)))
+        return fail(RSORT_BAD_ARGUMENT, "cache scores overlap the lengths");
     st = check_alignment(addr(d_weights), eb, "attention weights alignment");
     if (st == RSORT_OK) st = check_alignment(addr(d_scores), 4, "cache scores alignment");
     if (st == RSORT_OK) st = check_alignment(addr(d_lengths), 4, "cache lengths alignment");
@@ -749,8 +755,8 @@ rsort_status rsort_cache_select(const float *d_scores, size_t score_stride_b,
     if (!apart(kept_n, lengths))
         return fail(RSORT_BAD_ARGUMENT, "kept lengths overlap the lengths");
     Strided scores{};
-    if (!strided(d_scores, 4, {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}},
-                 &scores))
+    if (!strided(d_scores, 4,
+                 {{capacity, 4}, {heads, score_stride_h * 4}, {batch, score_stride_b * 4}}, &scores))
         return fail(RSORT_SIZE_OVERFLOW, "cache score strides");
     if (!apart(kept, scores) || !apart(kept_n, scores) || !apart(kept, kept_n) ||
         !apart(kept, lengths))
@@ -797,7 +803,8 @@ rsort_status rsort_cache_compact(const rsort_cache_rows *caches, size_t ncaches,
     st = check_alignment(addr(d_kept) | addr(d_kept_lengths), 4, "cache selection alignment");
     if (st != RSORT_OK) return st;
     const size_t bh = batch * heads;
-    const Strided kept = packed(d_kept, bh * budget * 4), kept_n = packed(d_kept_lengths, batch * 4);
+    const Strided kept = packed(d_kept, bh * budget * 4);
+    const Strided kept_n = packed(d_kept_lengths, batch * 4);
     Strided in[RSORT_MAX_CACHES], out[RSORT_MAX_CACHES];
     bool in_place = false;
     for (size_t i = 0; i < ncaches; ++i) {

@@ -177,3 +177,15 @@ def test_rows_of_one_allocation_that_share_a_byte_are_refused():
         rows = [cache(**view(0, 64, 0x100000), **into(0, 0x100000)),
                 cache(**view(offset, 32, 0x100000), **into(offset, 0x100000))]
         assert compact_status(*rows) == BAD
+
+
+# float32 weights [2, 4, 1, 64] at 0x10000 take 2 KB, totals [2, 2, 64] 1 KB
+@pytest.mark.parametrize("change", [
+    dict(scores=0x10000), dict(scores=0x107fc), dict(scores=0x10000 - 0x3fc),
+    dict(scores=0x1004 - 0x400), dict(scores=0x1004),        # over the lengths
+    dict(lengths=0x20000), dict(lengths=0x203fc),
+    # totals between the weights' heads, 96 apart, over the last of 32 weights
+    dict(sb=4 * 96, sh=96, scores=0x10000 + 4 * 31, score_b=4 * 96, score_h=96, capacity=32)])
+def test_add_refuses_totals_over_what_it_reads(change):
+    assert add_status(**change) == BAD
+    assert _lib.last_error().status == BAD

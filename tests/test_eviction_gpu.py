@@ -354,3 +354,17 @@ def test_compact_of_unequal_rows_in_one_allocation(H, widths, in_place):
     eviction.device_cache_compact(launch(), torch.from_numpy(kept).cuda(),
                                   torch.from_numpy(n).cuda(), src, None if in_place else dst)
     assert torch.equal(to, want)
+
+
+def test_totals_beside_the_weights_in_one_allocation():
+    rng = np.random.default_rng(12)
+    B, H, G, S = 3, 2, 2, 70
+    both = torch.from_numpy(rng.random((B, H * G + H, S)).astype(np.float32)).cuda()
+    before = both.clone()
+    w, scores = both[:, :H * G], both[:, H * G:]
+    eviction.device_attention_weight_add(launch(), w, scores, lengths_of([70, 0, 33]))
+    want = before.double()
+    for b, n in enumerate([70, 0, 33]):
+        want[b, H * G:, :n] += before[b, :H * G, :n].double().view(H, G, n).sum(1)
+    assert torch.equal(w, before[:, :H * G])
+    assert ((both.double() - want).abs() <= 4 * 2.0**-24 * want).all()
