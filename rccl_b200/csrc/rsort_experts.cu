@@ -884,13 +884,15 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
                              "expert weights alignment");
     if (st != RSORT_OK) return st;
     // Without weight gradients the rows are not read.
-    if (!apart(grad_rows, grad_out) || (d_grad_weights && !apart(grad_rows, rows)))
+    const size_t weight_bytes = size_t(p.tokens) * p.top_k * wb;
+    const Strided weights = packed(d_weights, d_weights ? weight_bytes : 0);
+    if (!apart(grad_rows, grad_out) || !apart(grad_rows, weights) ||
+        (d_grad_weights && !apart(grad_rows, rows)))
         return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
     if (d_grad_weights) {
-        const size_t weight_bytes = size_t(p.tokens) * p.top_k * wb;
         const Strided out = packed(d_grad_weights, weight_bytes);
         if (!apart(out, grad_out) || !apart(out, rows) || !apart(out, grad_rows) ||
-            (d_weights && !apart(out, packed(d_weights, weight_bytes))))
+            !apart(out, weights))
             return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap another buffer");
     }
     int sms = 0;

@@ -215,3 +215,16 @@ def test_python_refusals():
     for top_k in (0, 1025):
         with pytest.raises(BadArgument):
             experts.device_expert_plan(CPU, 4, top_k, 4)
+
+
+@pytest.mark.parametrize("weights,grad_rows,stride", [
+    (0x30000, 0x30000, 16), (0x30000, 0x3001c, 16), (0x30000, 0x30000 - 0x1fc, 16),
+    # weights in a gap between gradient rows but for their last byte's word
+    (0x40000 + 64, 0x40000, 16 + 7)])
+def test_gradient_rows_over_the_weights_are_refused(weights, grad_rows, stride):
+    """8 weights of 4 bytes; 8 gradient rows of 64 bytes.  CTAs go on reading
+    weights while others write rows."""
+    for grad_weights in (None, 0x60000):
+        assert L.rsort_expert_combine_backward(
+            plan_args(), F32, 0x10000, 16, 0x20000, 16, weights, F32, grad_rows, stride,
+            grad_weights, 16, 1, None) == _lib.RSORT_BAD_ARGUMENT
