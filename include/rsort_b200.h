@@ -544,8 +544,8 @@ rsort_status rsort_keys_static(rsort_key_t key, int descending, void *d_keys, si
  *                         slots.  Either output may be null.
  * Row types are f32, f16 or bf16, weights any of them (tokens x top_k,
  * contiguous); strides of typed rows are in elements.  Input rows may have any
- * stride (0: one row for all); output rows must not overlap one another or an
- * input.  `rows` and `grad_rows` hold nrows rows.
+ * stride (0: one row for all); output rows must not overlap one another, an
+ * input or the plan.  `rows` and `grad_rows` hold nrows rows.
  * ------------------------------------------------------------------------- */
 #define RSORT_MAX_EXPERTS 1024
 #define RSORT_MAX_EXPERT_ALIGN 65536

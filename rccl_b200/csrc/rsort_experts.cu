@@ -664,6 +664,13 @@ rsort_status check_plan(const rsort_expert_plan *p, Plan *out) {
     return RSORT_OK;
 }
 
+// CTAs read the plan while others write.
+bool apart_from_plan(const Plan &p, const Strided &out) {
+    return apart(out, packed(p.row_of_slot, size_t(p.tokens) * p.top_k * 4)) &&
+           apart(out, packed(p.offsets, (size_t(p.experts) + 1) * 4)) &&
+           apart(out, packed(p.counts, size_t(p.experts) * 4));
+}
+
 }  // namespace
 
 extern "C" {
@@ -764,6 +771,7 @@ rsort_status rsort_expert_gather(const rsort_expert_plan *plan, const void *d_x,
         return fail(RSORT_SIZE_OVERFLOW, "expert rows");
     if (!apart(x, rows))
         return fail(RSORT_BAD_ARGUMENT, "expert rows overlap the tokens");
+    if (!apart_from_plan(p, rows)) return fail(RSORT_BAD_ARGUMENT, "expert rows overlap the plan");
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
@@ -817,6 +825,8 @@ rsort_status rsort_expert_combine(const rsort_expert_plan *plan, rsort_key_t typ
     const size_t weight_bytes = size_t(p.tokens) * p.top_k * real_bytes(weight_type);
     if (d_weights && !apart(packed(d_weights, weight_bytes), out))
         return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the weights");
+    if (!apart_from_plan(p, out))
+        return fail(RSORT_BAD_ARGUMENT, "expert output overlaps the plan");
     int sms = 0;
     st = current_sm_count(&sms);
     if (st != RSORT_OK) return st;
@@ -887,12 +897,12 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
     const size_t weight_bytes = size_t(p.tokens) * p.top_k * wb;
     const Strided weights = packed(d_weights, d_weights ? weight_bytes : 0);
     if (!apart(grad_rows, grad_out) || !apart(grad_rows, weights) ||
-        (d_grad_weights && !apart(grad_rows, rows)))
+        (d_grad_weights && !apart(grad_rows, rows)) || !apart_from_plan(p, grad_rows))
         return fail(RSORT_BAD_ARGUMENT, "expert gradient rows overlap an input");
     if (d_grad_weights) {
         const Strided out = packed(d_grad_weights, weight_bytes);
         if (!apart(out, grad_out) || !apart(out, rows) || !apart(out, grad_rows) ||
-            !apart(out, weights))
+            !apart(out, weights) || !apart_from_plan(p, out))
             return fail(RSORT_BAD_ARGUMENT, "expert weight gradients overlap another buffer");
     }
     int sms = 0;

@@ -228,3 +228,20 @@ def test_gradient_rows_over_the_weights_are_refused(weights, grad_rows, stride):
         assert L.rsort_expert_combine_backward(
             plan_args(), F32, 0x10000, 16, 0x20000, 16, weights, F32, grad_rows, stride,
             grad_weights, 16, 1, None) == _lib.RSORT_BAD_ARGUMENT
+
+
+# the plan's arrays: 8 slots' rows at 0x1000, 4 offsets at 0x2000, 3 counts at 0x3000
+@pytest.mark.parametrize("at", [0x1000, 0x101c, 0x2000, 0x200c, 0x3000, 0x3008])
+def test_outputs_over_the_plan_are_refused(at):
+    """Whether the output starts there or ends there."""
+    for rows, tokens in ((at, at), (at + 4 - 8 * 64, at + 4 - 4 * 64)):
+        assert L.rsort_expert_gather(plan_args(), 0x10000, 64, rows, 64, 64, 1,
+                                     None) == _lib.RSORT_BAD_ARGUMENT
+        for weights in (None, 0x20000):
+            assert L.rsort_expert_combine(plan_args(), F32, 0x10000, 16, weights, F32, tokens, 16,
+                                          16, None) == _lib.RSORT_BAD_ARGUMENT
+        for grad_rows, grad_weights in ((rows, None), (rows, 0x60000), (0x50000, at),
+                                        (None, at), (None, at + 4 - 32)):
+            assert L.rsort_expert_combine_backward(
+                plan_args(), F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, grad_rows, 16,
+                grad_weights, 16, 1, None) == _lib.RSORT_BAD_ARGUMENT
