@@ -142,26 +142,33 @@ def _rows(role: str, t: torch.Tensor, count: int, width: int, at_least: bool = F
     return stride
 
 
-def _weights(t: torch.Tensor, plan: ExpertPlan, role: str = "expert weights") -> int:
-    code = real_code(t.dtype)
+def _slots(role: str, t: torch.Tensor, plan: ExpertPlan) -> None:
+    """One entry a slot in the slots' order: (tokens, top_k), with any leading
+    dimensions for the tokens, or flat; of any shape when top_k is 1."""
+    shape = t.shape
     if t.numel() != plan.tokens * plan.top_k:
         raise LengthMismatch(role, plan.tokens * plan.top_k, t.numel())
+    if len(shape) > 1 and shape[-1] != plan.top_k > 1:
+        raise LengthMismatch(role + " of a token", plan.top_k, shape[-1])
     if not t.is_contiguous():
         raise BadArgument(f"{role} must be contiguous")
+
+
+def _weights(t: torch.Tensor, plan: ExpertPlan, role: str = "expert weights") -> int:
+    code = real_code(t.dtype)
+    _slots(role, t, plan)
     return code
 
 
 def device_expert_sort(launch: Launch, expert_ids: torch.Tensor, plan: ExpertPlan) -> None:
     """Sort the slots of expert_ids (tokens, top_k; int32 or int64) stably by
-    expert into the plan."""
+    expert into the plan.  Ids and weights may also be (batch, length, top_k) or
+    flat, as long as their slots are in that order."""
     _on(launch, expert_ids, plan.row_of_slot)
     code = ID_TYPES.get(expert_ids.dtype)
     if code is None:
         raise BadArgument(f"expert ids of {expert_ids.dtype} (int32 or int64)")
-    if expert_ids.numel() != plan.tokens * plan.top_k:
-        raise LengthMismatch("expert ids", plan.tokens * plan.top_k, expert_ids.numel())
-    if not expert_ids.is_contiguous():
-        raise BadArgument("expert ids must be contiguous")
+    _slots("expert ids", expert_ids, plan)
     call(launch, _lib.lib().rsort_expert_sort, code, expert_ids.data_ptr(), *plan.sort_args)
 
 

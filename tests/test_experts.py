@@ -245,3 +245,19 @@ def test_outputs_over_the_plan_are_refused(at):
             assert L.rsort_expert_combine_backward(
                 plan_args(), F32, 0x10000, 16, 0x20000, 16, 0x30000, F32, grad_rows, 16,
                 grad_weights, 16, 1, None) == _lib.RSORT_BAD_ARGUMENT
+
+
+def test_ids_and_weights_in_another_order_are_refused():
+    """(top_k, tokens) has as many entries, but its slots are in another order."""
+    plan = plan_on_cpu(tokens=6, top_k=2)
+    x, rows = torch.zeros(6, 8), torch.zeros(plan.rows, 8)
+    for shape in ((2, 6), (3, 4), (12, 1), (1, 12), (2, 2, 3)):
+        ids, w = torch.zeros(shape, dtype=torch.int64), torch.zeros(shape)
+        with pytest.raises(LengthMismatch):
+            experts.device_expert_sort(CPU, ids, plan)
+        with pytest.raises(LengthMismatch):
+            experts.device_expert_combine(CPU, rows, w, plan, x)
+        with pytest.raises(LengthMismatch):
+            experts.device_expert_combine_backward(CPU, x, rows, w, plan, rows, None)
+        with pytest.raises(LengthMismatch):
+            experts.device_expert_combine_backward(CPU, x, rows, torch.zeros(6, 2), plan, rows, w)

@@ -477,3 +477,23 @@ def test_rows_and_outputs_side_by_side_in_one_allocation(dtype, width):
     got_w = torch.full_like(s.w, 44)
     experts.device_expert_combine_backward(s.lau, s.grad, left, s.w, s.plan, right, got_w)
     assert torch.equal(right[:s.plan.rows], grad_rows) and torch.equal(got_w, grad_w)
+
+
+@pytest.mark.parametrize("top_k", [1, 3])
+def test_slots_of_a_batch_of_sequences_and_in_one_row(top_k):
+    """Ids and weights (batch, length, top_k), or flat: the slots in order."""
+    rng = np.random.default_rng(top_k)
+    batch, length, count, width = 4, 5, 6, 16
+    ids = make_ids(rng, batch * length, top_k, count, "mixed", torch.int64)
+    s = Step(17, batch * length, top_k, count, 1, width, torch.float32, torch.float32)
+    flat = [(-1,)] + ([(batch, length), (1, batch * length)] if top_k == 1 else [])
+    for shape in [(batch, length, top_k), (batch * length, top_k)] + flat:
+        experts.device_expert_sort(s.lau, ids.cuda().view(shape), s.plan)
+        check_plan(s.plan, ids, count, 1)
+    s = Step(17, batch * length, top_k, count, 1, width, torch.float32, torch.float32)
+    want = s.out(s.tokens)
+    experts.device_expert_combine(s.lau, s.rows, s.w, s.plan, want)
+    for shape in [(batch, length, top_k)] + flat:
+        y = s.out(s.tokens)
+        experts.device_expert_combine(s.lau, s.rows, s.w.view(shape), s.plan, y)
+        assert torch.equal(y, want)
