@@ -18,6 +18,7 @@ slots: they take no row, add nothing and get no gradient.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -51,13 +52,15 @@ def expert_rows(tokens: int, top_k: int, experts: int, align: int = 1) -> int:
     return rows
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class ExpertPlan:
     """Where every slot goes, filled by device_expert_sort.
 
     row_of_slot (tokens, top_k): a slot's row, -1 when dropped; slot_of_row
     (rows): a row's slot, -1 in padding; offsets (experts + 1): every expert's
-    first row; counts (experts): its slots.  All int32 on the device."""
+    first row; counts (experts): its slots.  All int32 on the device; scratch is
+    the sort's, uint8.  The calls take the arrays' addresses from here, so a
+    plan keeps the arrays that it was made with."""
     tokens: int
     top_k: int
     experts: int
@@ -70,14 +73,29 @@ class ExpertPlan:
     scratch: torch.Tensor
 
     def __post_init__(self):
-        self._args = _lib.ExpertPlanArgs(
+        for name, t, shape in (("row_of_slot", self.row_of_slot, (self.tokens, self.top_k)),
+                               ("slot_of_row", self.slot_of_row, (self.rows,)),
+                               ("offsets", self.offsets, (self.experts + 1,)),
+                               ("counts", self.counts, (self.experts,))):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise BadArgument(f"expert plan {name} must be contiguous int32")
+            if t.shape != shape:
+                raise LengthMismatch("expert plan " + name, math.prod(shape), t.numel())
+        if self.scratch.dtype != torch.uint8 or not self.scratch.is_contiguous():
+            raise BadArgument("expert plan scratch must be contiguous uint8")
+        for t in (self.slot_of_row, self.offsets, self.counts, self.scratch):
+            if t.device != self.row_of_slot.device:
+                raise ContextMismatch(f"expert plan on {self.row_of_slot.device} and {t.device}")
+        args = _lib.ExpertPlanArgs(
             self.row_of_slot.data_ptr(), self.offsets.data_ptr(), self.counts.data_ptr(),
             self.tokens, self.top_k, self.experts, self.rows)
-        self.args = ctypes.byref(self._args)
-        self.sort_args = (self.tokens * self.top_k, self.experts, self.align,
-                          self.row_of_slot.data_ptr(), self.slot_of_row.data_ptr(), self.rows,
-                          self.offsets.data_ptr(), self.counts.data_ptr(),
-                          self.scratch.data_ptr(), self.scratch.numel())
+        sort_args = (self.tokens * self.top_k, self.experts, self.align,
+                     self.row_of_slot.data_ptr(), self.slot_of_row.data_ptr(), self.rows,
+                     self.offsets.data_ptr(), self.counts.data_ptr(),
+                     self.scratch.data_ptr(), self.scratch.numel())
+        for name, value in (("_args", args), ("args", ctypes.byref(args)),
+                            ("sort_args", sort_args)):
+            object.__setattr__(self, name, value)
 
 
 def device_expert_plan(launch: Launch, tokens: int, top_k: int, experts: int,

@@ -1,6 +1,7 @@
 """CPU tests of the expert routing's sizing and refusals: every call here is
 sized or rejected on the host before any device work."""
 import ctypes
+import dataclasses
 
 import pytest
 import torch
@@ -261,3 +262,40 @@ def test_ids_and_weights_in_another_order_are_refused():
             experts.device_expert_combine_backward(CPU, x, rows, w, plan, rows, None)
         with pytest.raises(LengthMismatch):
             experts.device_expert_combine_backward(CPU, x, rows, torch.zeros(6, 2), plan, rows, w)
+
+
+ARRAYS = ("row_of_slot", "slot_of_row", "offsets", "counts", "scratch")
+
+
+def test_a_plan_keeps_its_arrays():
+    """The calls take the arrays' addresses from the plan once, so none can be
+    replaced in place; a plan with another array is another plan."""
+    plan = plan_on_cpu()
+    for name in ARRAYS:
+        other = getattr(plan, name).clone()
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            setattr(plan, name, other)
+        assert getattr(plan, name) is not other
+        fresh = dataclasses.replace(plan, **{name: other})
+        assert getattr(fresh, name) is other
+        where = [getattr(fresh, n).data_ptr() for n in ARRAYS]
+        args = fresh._args
+        assert [args.row_of_slot, args.offsets, args.counts] == [where[0], where[2], where[3]]
+        a = fresh.sort_args
+        assert [a[3], a[4], a[6], a[7], a[8]] == where
+    with pytest.raises(dataclasses.FrozenInstanceError):
+        plan.tokens = 5
+
+
+@pytest.mark.parametrize("name", ARRAYS)
+def test_a_plan_of_wrong_arrays_is_refused(name):
+    """The kernels trust the arrays' sizes."""
+    plan = plan_on_cpu()
+    t = getattr(plan, name)
+    wide = torch.zeros(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype)
+    bad = [(t.to(torch.int64), BadArgument), (wide[..., ::2], BadArgument)]
+    if name != "scratch":  # whose size every sort checks
+        bad += [(t[:-1].contiguous(), LengthMismatch), (wide, LengthMismatch)]
+    for other, error in bad:
+        with pytest.raises(error):
+            dataclasses.replace(plan, **{name: other})
