@@ -590,7 +590,9 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
  *       weights[b, h * group + g, q, s] over g < group and q < queries, in
  *       fp32, for s < lengths[b]; other totals are left as they are.  With
  *       causal the queries are the last ones of the sequence: query q sees
- *       s <= lengths[b] - queries + q, and what it does not see is not read.
+ *       s <= lengths[b] - queries + q.  What is not seen, or lies behind
+ *       lengths[b], adds nothing whatever it holds (NaN too), but may be read
+ *       within the row's capacity, so nothing may write it meanwhile.
  *       Weights are f32, f16 or bf16; strides in elements, positions next to
  *       one another.  Null lengths: every position is in use.  The totals must
  *       not share a byte with the weights or the lengths.

@@ -72,7 +72,8 @@ def device_attention_weight_add(launch: Launch, weights: torch.Tensor, scores: t
     weights (batch, query heads, queries, capacity), or (batch, query heads,
     capacity) for a single token: float32, float16 or bfloat16; query head
     h * group + g reads cache head h.  With causal the queries are the last
-    ones of each sequence and what a query does not see is not read."""
+    ones of each sequence.  What is not seen, or lies behind a length, adds
+    nothing whatever it holds, but may be read: nothing may write it meanwhile."""
     _on(launch, weights, scores, lengths)
     if weights.dim() == 3:
         weights = weights.unsqueeze(2)

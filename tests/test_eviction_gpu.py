@@ -368,3 +368,22 @@ def test_totals_beside_the_weights_in_one_allocation():
         want[b, H * G:, :n] += before[b, :H * G, :n].double().view(H, G, n).sum(1)
     assert torch.equal(w, before[:, :H * G])
     assert ((both.double() - want).abs() <= 4 * 2.0**-24 * want).all()
+
+
+@pytest.mark.parametrize("Q,G,S", [(1, 2, 40), (3, 2, 1000), (40, 4, 520), (41, 1, 333)])
+def test_unseen_weights_add_nothing_whatever_they_hold(Q, G, S):
+    """Infinities of both signs, NaN and the type's largest and lowest values in
+    every place that a query does not see give the same bits as zeros."""
+    rng = np.random.default_rng(Q)
+    B, lens = 3, [S, S // 2 + 1, 2]
+    w = torch.from_numpy(rng.random((B, G, Q, S)).astype(np.float32)).bfloat16()
+    seen = torch.from_numpy(visible(B, Q, S, lens, True))[:, None].expand(w.shape)
+    odd = [float("inf"), -float("inf"), NAN, torch.finfo(w.dtype).max, torch.finfo(w.dtype).min]
+    got = []
+    for fill in [torch.zeros(w.shape, dtype=w.dtype),
+                 torch.tensor(odd, dtype=w.dtype)[torch.randint(5, w.shape)]]:
+        scores = torch.ones(B, 1, S, device="cuda")
+        eviction.device_attention_weight_add(launch(), torch.where(seen, w, fill).cuda(), scores,
+                                             lengths_of(lens), causal=True)
+        got.append(scores.cpu())
+    assert torch.equal(*got)
