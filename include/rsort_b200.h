@@ -606,9 +606,11 @@ rsort_status rsort_expert_combine_backward(const rsort_expert_plan *plan, rsort_
  *       dst[b, h, j] = src[b, h, kept[b, h, j]] for j < kept_lengths[b], for
  *       up to RSORT_MAX_CACHES arrays of rows in one launch (keys, values,
  *       totals, scales).  Later rows are left as they are.  src == dst (with
- *       equal strides, for all arrays) compacts in place and takes ascending
- *       kept positions, as rsort_cache_select writes them; otherwise no dst
- *       may overlap a src.  Positions outside 0..capacity-1 are skipped.
+ *       equal strides, for all arrays) compacts in place and takes strictly
+ *       ascending kept positions, as rsort_cache_select writes them (a position
+ *       below its own place j does not move); otherwise no dst may overlap a
+ *       src, and positions may be in any order and repeat.  Positions outside
+ *       0..capacity-1 are skipped.
  *       Strides are in bytes, a row's bytes are next to one another.
  * ------------------------------------------------------------------------- */
 #define RSORT_MAX_CACHES 8

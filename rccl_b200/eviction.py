@@ -134,7 +134,8 @@ def device_cache_compact(launch: Launch, kept: torch.Tensor, kept_lengths: torch
     of any element type and any strides but neighbouring elements in a row
     (pass a transposed view of a (batch, capacity, heads, width) cache).
     Without destinations, or with the sources themselves, the cache is
-    compacted in place by ascending kept positions."""
+    compacted in place by strictly ascending kept positions (as selected);
+    otherwise they may be in any order and repeat."""
     if destinations is None:
         destinations = sources
     if len(sources) != len(destinations):

@@ -387,3 +387,25 @@ def test_unseen_weights_add_nothing_whatever_they_hold(Q, G, S):
                                              lengths_of(lens), causal=True)
         got.append(scores.cpu())
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("D", [1, 64, 129])
+def test_compact_out_of_place_in_any_order_with_repeats(D):
+    rng = np.random.default_rng(D)
+    B, H, S, budget = 2, 3, 60, 41
+    k = torch.from_numpy(rng.normal(size=(B, H, S, D))).half().cuda()
+    kept = rng.integers(0, S, (B, H, budget)).astype(np.int32)
+    kept[:, :, 1], kept[:, :, 2] = kept[:, :, 0], kept[:, :, 0]
+    n = np.array([budget, 7], np.int32)
+    dst = torch.full((B, H, budget, D), 5, dtype=k.dtype, device="cuda")
+    want = moved(k.cpu(), kept, n, dst.cpu())
+    eviction.device_cache_compact(launch(), torch.from_numpy(kept).cuda(),
+                                  torch.from_numpy(n).cuda(), [k], [dst])
+    assert torch.equal(dst.cpu(), want)
+
+
+def test_in_place_a_position_below_its_place_does_not_move():
+    kept = torch.tensor([[[0, 0, 4, 5, 5, 1]]], dtype=torch.int32, device="cuda")
+    k = torch.arange(8, dtype=torch.float32, device="cuda").view(1, 1, 8, 1) + 1
+    eviction.device_cache_compact(launch(), kept, lengths_of([6]), [k])
+    assert k.view(-1).tolist() == [1, 2, 5, 6, 6, 6, 7, 8]
