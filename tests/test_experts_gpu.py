@@ -15,6 +15,7 @@ from rccl_b200 import cub, experts
 pytestmark = pytest.mark.gpu
 
 HALF = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+NAN = float("nan")
 TINY = {torch.float32: 2.0**-149, torch.float16: 2.0**-24, torch.bfloat16: 2.0**-133}
 
 
@@ -497,3 +498,114 @@ def test_slots_of_a_batch_of_sequences_and_in_one_row(top_k):
         y = s.out(s.tokens)
         experts.device_expert_combine(s.lau, s.rows, s.w.view(shape), s.plan, y)
         assert torch.equal(y, want)
+
+
+# Tokens for several trips of every CTA of the combine and of its gradient, the
+# last one ragged: at most five CTAs of 256 threads an SM stay resident, and a
+# token takes from 2 threads (128 tokens a CTA) to 256.
+MANY = [(200_003, 1, 8, torch.bfloat16, torch.float32),
+        (100_003, 8, 4, torch.float32, torch.float32),
+        (60_001, 2, 64, torch.bfloat16, torch.bfloat16),
+        (15_001, 3, 33, torch.float32, torch.float32),
+        (12_001, 17, 264, torch.bfloat16, torch.float32),
+        (13_003, 3, 2056, torch.bfloat16, torch.float32),
+        (7_001, 5, 512, torch.bfloat16, torch.float32),
+        (4_003, 4, 1024, torch.float16, torch.float16),
+        (3_001, 1, 1001, torch.float32, torch.float32),
+        (3_001, 2, 1001, torch.float32, torch.bfloat16),
+        (3_001, 9, 1001, torch.float32, torch.float32),
+        (3_001, 6, 4096, torch.bfloat16, torch.float32),
+        (3_001, 8, 2056, torch.float16, torch.float32),
+        (3_001, 8, 4096, torch.bfloat16, torch.bfloat16)]
+
+
+def close_here(got, want, mag, terms, dtype):
+    tol = (terms + 1) * 2.0**-24 * mag
+    tol = tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype]
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("tokens,top_k,width,dtype,wdtype", MANY)
+def test_combine_and_gradients_of_many_tokens(tokens, top_k, width, dtype, wdtype):
+    """CTAs that work on token after token, the next one's slots held while
+    this one is summed; rows that no slot uses hold NaN, and two runs are equal
+    bit by bit."""
+    count, align = 12, 16
+    rng = np.random.default_rng(tokens + width)
+    ids = make_ids(rng, tokens, top_k, count, "mixed", torch.int64)
+    lau, plan = sort(ids, count, align)
+    check_plan(plan, ids, count, align)
+    g = torch.Generator(device="cuda").manual_seed(width)
+
+    def normal(*shape, dtype=dtype):
+        return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+    rows, grad = normal(plan.rows, width), normal(tokens, width)
+    rows[plan.slot_of_row < 0] = NAN
+    w = normal(tokens, top_k, dtype=wdtype)
+    w[plan.row_of_slot < 0] = NAN
+
+    slots = torch.nonzero(plan.row_of_slot.view(-1) >= 0).view(-1)
+    at, token = plan.row_of_slot.view(-1)[slots].long(), slots // top_k
+    w64 = w.double().view(-1)[slots].unsqueeze(1)
+
+    def sums(terms):
+        out = torch.zeros(2, tokens, width, dtype=torch.float64, device="cuda")
+        return out[0].index_add_(0, token, terms), out[1].index_add_(0, token, terms.abs())
+
+    def twice(make, call):
+        """The outputs of a call, which a second one gives again."""
+        first, second = make(), make()
+        call(*first)
+        call(*second)
+        for a, b in zip(first, second):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        return first
+
+    def filled(n, like=rows, to=33):
+        return torch.full((n, like.shape[1]), to, dtype=like.dtype, device="cuda")
+
+    y, = twice(lambda: [filled(tokens)],
+               lambda y: experts.device_expert_combine(lau, rows, w, plan, y))
+    close_here(y, *sums(rows[at].double() * w64), top_k, dtype)
+    grad_x, = twice(lambda: [filled(tokens)],
+                    lambda x: experts.device_expert_gather_backward(lau, rows, plan, x))
+    close_here(grad_x, *sums(rows[at].double()), top_k, dtype)
+
+    grad_rows, grad_w = twice(
+        lambda: [filled(plan.rows), filled(tokens, w, 44)],
+        lambda a, b: experts.device_expert_combine_backward(lau, grad, rows, w, plan, a, b))
+    want = torch.full((plan.rows, width), 33.0, dtype=torch.float64, device="cuda")
+    want[:int(plan.offsets[-1])] = 0
+    want[at] = grad.double()[token] * w64
+    close_here(grad_rows, want, want.abs(), 0, dtype)
+    terms = grad.double()[token] * rows[at].double()
+    dots = torch.zeros(2, tokens * top_k, dtype=torch.float64, device="cuda")
+    dots[0, slots], dots[1, slots] = terms.sum(1), terms.abs().sum(1)
+    close_here(grad_w.view(-1), dots[0], dots[1], width, wdtype)
+    only, = twice(lambda: [filled(tokens, w, 44)],
+                  lambda b: experts.device_expert_combine_backward(lau, grad, rows, w, plan, None, b))
+    assert torch.equal(only, grad_w)
+
+    moved = filled(plan.rows)
+    experts.device_expert_gather(lau, grad, plan, moved)
+    want.fill_(33)
+    want[:int(plan.offsets[-1])] = 0
+    want[at] = grad.double()[token]
+    assert torch.equal(moved.double(), want)
+
+
+@pytest.mark.parametrize("align", [1, 4096])
+def test_padding_of_other_alignments(align):
+    """No padding at all, and padding rows by the thousand."""
+    s = Step(5, 21, 2, 3, align, 40, torch.float16, torch.float32, kind="uniform")
+    rows, grad_rows = s.out(s.plan.rows), s.out(s.plan.rows)
+    experts.device_expert_gather(s.lau, s.grad, s.plan, rows)
+    experts.device_expert_combine_backward(s.lau, s.grad, s.rows, s.w, s.plan, grad_rows, None)
+    end = int(s.offsets[-1])
+    padding = torch.from_numpy(s.slot_of_row[:end] < 0).cuda()
+    for out in (rows, grad_rows):
+        assert (out[:end][padding] == 0).all() and (out[end:] == 33).all()
+    used = torch.from_numpy(s.row_of_slot[s.used]).cuda()
+    assert torch.equal(rows[used], s.grad[torch.from_numpy(s.used // 2).cuda()])
