@@ -60,18 +60,26 @@ struct Axis {
     size_t count, stride;
 };
 struct Strided {
-    uintptr_t first = 0, last = 0;
-    size_t bytes = 0;
-    Axis axis[4] = {};
-    int axes = 0;
+    uintptr_t first, last;
+    size_t bytes;
+    int axes;
+    Axis axis[4];
 };
+
+// `bytes` next to one another.
+inline Strided packed(const void *p, size_t bytes) {
+    Strided r;
+    r.first = addr(p);
+    r.last = r.first + bytes;
+    r.bytes = bytes;
+    r.axes = 0;
+    return r;
+}
 
 // False when an offset could wrap.
 inline bool strided(const void *p, size_t bytes, std::initializer_list<Axis> axes, Strided *out) {
-    Strided r;
-    r.first = r.last = addr(p);
-    r.bytes = bytes;
-    size_t extent = bytes;
+    Strided &r = *out;
+    r = packed(p, bytes);
     bool empty = bytes == 0;
     for (const Axis &x : axes) {
         if (!rows_fit(x.count, x.stride, bytes)) return false;
@@ -80,18 +88,10 @@ inline bool strided(const void *p, size_t bytes, std::initializer_list<Axis> axe
         int at = r.axes++;
         for (; at > 0 && r.axis[at - 1].stride > x.stride; --at) r.axis[at] = r.axis[at - 1];
         r.axis[at] = x;
-        extent += (x.count - 1) * x.stride;
+        r.last += (x.count - 1) * x.stride;
     }
-    if (!empty) r.last += extent;
-    *out = r;
+    if (empty) r.last = r.first;
     return true;
-}
-
-// `bytes` next to one another.
-inline Strided packed(const void *p, size_t bytes) {
-    Strided r;
-    strided(p, bytes, {}, &r);
-    return r;
 }
 
 // No two items share a byte (sufficient: every stride spans what lies inside).
@@ -104,20 +104,17 @@ inline bool items_apart(const Strided &a) {
     return true;
 }
 
-// No item of one shares a byte with an item of the other (sufficient: their
-// spans are apart, or they lie side by side within some stride s of theirs, as
-// keys and values of one allocation do: axes whose strides are multiples of s
-// leave an address as it is modulo s, so each array covers one interval there).
-inline bool apart(const Strided &a, const Strided &b) {
-    if (a.first >= b.last || b.first >= a.last || a.first >= a.last || b.first >= b.last)
-        return true;
+// Both arrays lie within one interval each modulo some stride s of theirs, and
+// these are apart, as keys and values of one allocation are (axes whose strides
+// are multiples of s leave an address as it is modulo s).
+inline bool side_by_side(const Strided &a, const Strided &b) {
     const auto width = [](const Strided &x, size_t s) {
         size_t w = x.bytes;
         for (int i = 0; i < x.axes; ++i)
             if (x.axis[i].stride % s) w += (x.axis[i].count - 1) * x.axis[i].stride;
         return w;
     };
-    const auto side_by_side = [&](size_t s) {
+    const auto within = [&](size_t s) {
         if (s == 0) return false;
         const size_t wa = width(a, s), wb = width(b, s);
         const size_t d = b.first >= a.first ? (b.first - a.first) % s
@@ -125,10 +122,17 @@ inline bool apart(const Strided &a, const Strided &b) {
         return wa <= d && wb <= s - d;
     };
     for (int i = 0; i < a.axes; ++i)
-        if (side_by_side(a.axis[i].stride)) return true;
+        if (within(a.axis[i].stride)) return true;
     for (int i = 0; i < b.axes; ++i)
-        if (side_by_side(b.axis[i].stride)) return true;
+        if (within(b.axis[i].stride)) return true;
     return false;
+}
+
+// No item of one shares a byte with an item of the other (sufficient: their
+// spans are apart, or they lie side by side).
+inline bool apart(const Strided &a, const Strided &b) {
+    return a.first >= b.last || b.first >= a.last || a.first >= a.last || b.first >= b.last ||
+           side_by_side(a, b);
 }
 
 // Thread-block clusters: a word of CTA `rank`'s shared memory at the same

@@ -94,7 +94,7 @@ class ExpertPlan:
                      self.offsets.data_ptr(), self.counts.data_ptr(),
                      self.scratch.data_ptr(), self.scratch.numel())
         for name, value in (("_args", args), ("args", ctypes.byref(args)),
-                            ("sort_args", sort_args)):
+                            ("sort_args", sort_args), ("slots", (self.tokens, self.top_k))):
             object.__setattr__(self, name, value)
 
 
@@ -164,6 +164,8 @@ def _slots(role: str, t: torch.Tensor, plan: ExpertPlan) -> None:
     """One entry a slot in the slots' order: (tokens, top_k), with any leading
     dimensions for the tokens, or flat; of any shape when top_k is 1."""
     shape = t.shape
+    if shape == plan.slots and t.is_contiguous():
+        return
     if t.numel() != plan.tokens * plan.top_k:
         raise LengthMismatch(role, plan.tokens * plan.top_k, t.numel())
     if len(shape) > 1 and shape[-1] != plan.top_k > 1:
