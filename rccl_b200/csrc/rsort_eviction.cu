@@ -33,11 +33,15 @@ __device__ __forceinline__ uint32_t length_of(const int32_t *lengths, uint32_t b
 // CTAs of a cluster, whose sums meet in (distributed) shared memory in a fixed
 // order.  Two loads a thread in flight (four where rows are dealt out) at four
 // CTAs an SM were best: one query of 64 x 32 heads over 32 Ki positions, bf16
-// (201 MB), 33 us with 2 (6.0 TB/s), 38 with 4, 42 with 8; 256 queries of 2 x 32
-// heads over 16 Ki, causal (490 MB), 80 us (6.1 TB/s) with four CTAs an SM's worth
-// of work dealt out, 88 and 94 us with 8 and 16.  Tiles that some queries see only
-// in part are masked behind the reads: with a branch before each read their
-// CTAs ran twice as long as the others (110 us).
+// (201 MB), 33 us with 2, 38 with 4, 42 with 8 (36 us a call in a row, 5.5 TB/s);
+// 256 queries of 2 x 32 heads over 16 Ki, causal (490 MB), 80 us with four CTAs an
+// SM's worth of work dealt out, 88 and 94 us with 8 and 16 (83 us a call in a row,
+// 5.9 TB/s).  At four CTAs an SM the dealt-out form spills 64 to 72 bytes a thread
+// in 16-byte packs of two-byte elements.  Tiles that some queries see only in part
+// are masked behind the reads: with a branch before each read their CTAs ran twice
+// as long as the others (110 us).  Rows that 16 bytes do not divide leave fewer
+// bytes in flight: 32 x 32 heads of one query take 7.7 us a call over 8192
+// positions, 7.8 over 8188, 13 over 8190 and 17 over 8191.
 // ---------------------------------------------------------------------------
 constexpr uint32_t ADD_WARPS = 8;
 constexpr uint32_t ADD_BLOCK = ADD_WARPS * 32;
@@ -506,8 +510,9 @@ struct Walk {
 
 // Out of place: a CTA moves MOVE_BLOCK * MOVE_UNITS accesses; positions that
 // cannot be read do not move.  (64 heads to 2048 rows of 256 bytes, keys and
-// values, 139 MB: 18.5 us, 31 us with four accesses a thread and divisions by the
-// row's length for each.)
+// values, 139 MB: 18.5 us from a clean L2, which still holds part of the writes at
+// the end, 31 us with four accesses a thread and divisions by the row's length for
+// each; 24.5 us a call in a row, 5.5 TB/s.)
 template <typename U>
 __device__ __forceinline__ void move_out(const Rows &r, const int32_t *kept, const char *src,
                                          char *dst, uint32_t n, uint32_t capacity, uint32_t block) {

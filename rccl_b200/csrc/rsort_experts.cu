@@ -338,9 +338,9 @@ __device__ __forceinline__ void zero_padding(const Plan &p, uint32_t b, char *ro
 }
 
 // rows[row of slot] = x[t]: a token is read once and written to all of its rows,
-// so the kernel is bound by the writes (16 Ki tokens to 8 rows of 4096 bf16 and
-// the padding of 128 experts, 1.27 GB, 205 us: 6.2 TB/s; 8191 tokens to 6 rows
-// of 2048, 240 MB, 36 us: 6.6 TB/s).
+// so the kernel is bound by the writes (calls in a row: 16 Ki tokens to 8 rows of
+// 4096 bf16 and the padding of 128 experts, 1.28 GB, 211 us, 6.0 TB/s; 8191 tokens
+// to 6 rows of 2048, 241 MB, 40 us, 6.0 TB/s).
 template <typename U>
 __global__ void __launch_bounds__(ROW_BLOCK)
     expert_gather_kernel(const Plan p, const Shape s, const char *x, size_t x_stride, char *rows,
@@ -398,14 +398,16 @@ __host__ __device__ constexpr int columns_of(int elements, int slots) {
     return c;
 }
 
-// CTAs an SM: what the registers of `slots` reads in flight leave room for.
-// One more spills and one fewer leaves too few bytes in flight.  16 Ki tokens of
-// 8 rows of 4096 bf16 (1.21 GB): combine 204 / 184 / 186 us with 2 / 3 / 4
-// (6.5 TB/s; 237 us with a branch a row, 196 us with four rows at a time); its
-// gradient (2.28 GB) 407 / 405 / 485 us with 2 / 3 / 4 (5.6 TB/s).  4 Ki tokens of
-// 4 rows of 5120: 40 / 39 / 37 / 42 us with 3 / 4 / 5 / 6, 71 / 64 / 63 / 72 us
-// with 2 / 3 / 4 / 5.  Rings of asynchronous copies in shared memory were no
-// faster (194 and 466 us): they pay for the reads twice in shared memory.
+// CTAs an SM: what the registers of `slots` reads in flight leave room for.  As
+// chosen, one instance spills (4 bytes: combine, four f32 packs); with one CTA more,
+// 17 do (4 to 188 bytes).  Calls in a row, one CTA fewer / as chosen / one more:
+//   16 Ki tokens of 8 rows of 4096 bf16: combine (1.21 GB) 178 / 178 / 184 us
+//     (6.8 TB/s), its gradient (2.35 GB) 668 / 418 / 422 us (5.6 TB/s);
+//   8191 of 6 rows of 2048 bf16: 47 / 42 / 43 us, 114 / 94 / 92 us;
+//   4 Ki of 4 rows of 5120 f16: 38 / 35 / 40 us, 68 / 71 / 76 us.
+// Combine took 237 us instead with a branch a row and 196 us with four rows at a
+// time.  Rings of asynchronous copies in shared memory were no faster (194 and
+// 466 us): they pay for the reads twice in shared memory.
 constexpr int combine_ctas(int slots) { return slots <= 4 ? 5 : 4; }
 constexpr int backward_ctas(int elements, int slots) {
     return columns_of(elements, slots) > 1 ? 3 : slots <= 4 ? 4 : slots <= 6 ? 3 : 2;
@@ -618,7 +620,8 @@ __global__ void __launch_bounds__(ROW_BLOCK, backward_ctas(V, SLOTS))
 }
 
 // Calls f with the reads that a thread has in flight: all of a token's slots,
-// up to MOST_SLOTS.
+// up to MOST_SLOTS.  (With eight reads for six slots 8191 tokens of 2048 bf16 take
+// 44 us instead of 42, and the gradient, at one CTA an SM less, 129 instead of 94.)
 template <typename F> cudaError_t with_slots(uint32_t slots, F f) {
     if (slots <= 1) return f(std::integral_constant<int, 1>{});
     if (slots <= 2) return f(std::integral_constant<int, 2>{});
