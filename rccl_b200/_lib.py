@@ -109,6 +109,7 @@ class CompareTerm(ctypes.Structure):
 # limits of the expert routing and the cache eviction
 MAX_EXPERTS = 1024
 MAX_EXPERT_ALIGN = 65536
+MAX_EXPERT_SLOTS = 2**31 - 1
 MAX_CACHES = 8
 
 

@@ -117,8 +117,8 @@ def device_cache_select(launch: Launch, scores: torch.Tensor, lengths: Optional[
     _int32("kept lengths", kept_lengths, batch)
     if lengths is not None:
         _int32("cache lengths", lengths, batch)
-    if sinks < 0 or recent < 0:
-        raise BadArgument(f"{sinks} sinks, {recent} recent positions")
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise BadArgument(f"{sinks} sinks, {recent} recent positions, budget {budget}")
     score_b, score_h, _ = scores.stride()
     call(launch, _lib.lib().rsort_cache_select, scores.data_ptr(), score_b, score_h,
          None if lengths is None else lengths.data_ptr(), batch, heads, capacity, budget, sinks,

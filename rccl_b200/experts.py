@@ -45,8 +45,14 @@ def real_code(dtype: torch.dtype) -> int:
 
 def expert_rows(tokens: int, top_k: int, experts: int, align: int = 1) -> int:
     """Rows that hold every outcome of a sort of tokens x top_k slots."""
-    rows = _lib.lib().rsort_expert_rows(tokens * top_k, experts, align)
-    if rows == 0 and tokens * top_k:
+    rows = 0
+    # what a C size would wrap is out of range too
+    sized = (0 <= tokens <= _lib.MAX_EXPERT_SLOTS and 0 <= top_k and
+             tokens * top_k <= _lib.MAX_EXPERT_SLOTS and 1 <= experts <= _lib.MAX_EXPERTS and
+             1 <= align <= _lib.MAX_EXPERT_ALIGN)
+    if sized:
+        rows = _lib.lib().rsort_expert_rows(tokens * top_k, experts, align)
+    if not sized or (rows == 0 and tokens * top_k):
         raise BadArgument(f"no expert rows for {tokens} x {top_k} slots, {experts} experts "
                           f"(1..{_lib.MAX_EXPERTS}), align {align} (1..{_lib.MAX_EXPERT_ALIGN})")
     return rows
@@ -108,8 +114,6 @@ def device_expert_plan(launch: Launch, tokens: int, top_k: int, experts: int,
     rows = expert_rows(tokens, top_k, experts, align)
     lib = _lib.lib()
     nbytes = lib.rsort_expert_sort_scratch_bytes(tokens * top_k, experts)
-    if nbytes == 0:
-        raise BadArgument(f"{experts} experts (1..{_lib.MAX_EXPERTS}), align {align}")
     # One allocation for all arrays, each on 16 bytes.
     sizes = (nbytes // 4, tokens * top_k, rows, experts + 1, experts)
     starts, end = [], 0

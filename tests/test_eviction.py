@@ -189,3 +189,12 @@ def test_rows_of_one_allocation_that_share_a_byte_are_refused():
 def test_add_refuses_totals_over_what_it_reads(change):
     assert add_status(**change) == BAD
     assert _lib.last_error().status == BAD
+
+
+@pytest.mark.parametrize("sinks,recent", [(2**64, 0), (0, 2**64), (2**64 + 1, 1), (5, 0), (2, 3),
+                                          (0, 5)])
+def test_sinks_and_recent_positions_beyond_the_budget_are_refused(sinks, recent):
+    i32 = dict(dtype=torch.int32)
+    with pytest.raises(BadArgument):
+        eviction.device_cache_select(CPU, torch.zeros(2, 2, 8), None, torch.zeros(2, 2, 4, **i32),
+                                     torch.zeros(2, **i32), sinks, recent)

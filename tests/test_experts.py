@@ -299,3 +299,14 @@ def test_a_plan_of_wrong_arrays_is_refused(name):
     for other, error in bad:
         with pytest.raises(error):
             dataclasses.replace(plan, **{name: other})
+
+
+@pytest.mark.parametrize("tokens,top_k,count,align", [
+    (2**64 + 8, 1, 4, 1), (8, 2**64 + 1, 4, 1), (8, 1, 2**64 + 4, 1), (8, 1, 4, 2**64 + 1),
+    (2**31, 1, 4, 1), (-8, -1, 4, 1), (0, 2, 4, 0), (0, 2, 4, 65537), (0, 2, 0, 1), (8, 1, -4, 1)])
+def test_plan_sizes_out_of_range_are_refused(tokens, top_k, count, align):
+    """Sizes that a 64-bit word would wrap into range, and those of no slots."""
+    with pytest.raises(BadArgument):
+        experts.expert_rows(tokens, top_k, count, align)
+    with pytest.raises(BadArgument):
+        experts.device_expert_plan(CPU, tokens, top_k, count, align)
